@@ -678,6 +678,71 @@ int vlt5_decode_linear_tiles(int rows, int N, int K, int norm_folded);     /* no
  * f32 over <= 64 keys, d_kv in {16, 32, 64}; vlt5_attn_desc as for vlt5_attn_fwd with q_sb the sample stride of q, k_sb == v_sb,
  * k_st == v_st, bias [H][1][bias_k] (bias_q == 1), key_mask [B][Tk]; lse is not written. */
 int vlt5_decode_attn(const vlt5_attn_desc* d, void* stream);
+/* ---- the token-step in low precision: 4-bit weights (csrc/w4.hip), a paged key/value cache (csrc/paged.hip, csrc/paged_attn.hip) ----
+ * 4-bit weight [N, K]: `codes` u8 [N][K / 2], byte j of a row = k 2j in the low four bits, 2j + 1 in the high ones; a code is an e2m1
+ * number (bit 3 sign; 0 .5 1 1.5 2 3 4 6); `scales` bf16 [N][ceil(K / group)], group in {32, 64, 128} consecutive k (the last group of a
+ * row may be short).  K % 32 == 0, codes 16-byte aligned.
+ * vlt5_quant_w4 makes one from f32 or bf16 rows (one of the two pointers): scale = bf16(largest magnitude of the group / 6), code = the
+ * nearest e2m1 number to w / scale (f32, ties to the even code); a group with an infinity or a NaN gets the scale NaN. */
+int vlt5_quant_w4(const float* w_f32, const void* w_bf16, long long ldw, int N, int K, int group, void* codes, void* scales, void* stream);
+/* out[m, n] = act(alpha * sum_k x[m, k] value(code[n, k]) scale[n, k / group] (+ resid[m, n])), the vlt5_decode_linear of such a weight:
+ * rows <= VLT5_W4_MAX_ROWS, any N, x bf16 (rows 16-byte aligned), f32 sums, bf16 and / or f32 output.  `resid` may be `out_f32`. */
+#define VLT5_W4_MAX_ROWS 256
+typedef struct {
+    const void* x_bf16; long long ldx;
+    const void* codes; const void* scales; int rows, N, K, group;
+    float alpha;                                   /* 0 = 1 */
+    void* out_bf16; long long ld_out_bf16;
+    float* out_f32; long long ld_out_f32;
+    const float* resid; long long ld_resid;
+    int relu;
+} vlt5_decode_linear_w4_desc;
+int vlt5_decode_linear_w4(const vlt5_decode_linear_w4_desc* d, void* stream);
+
+/* The cache of one layer.  k, v: [n_pages][n_kv_heads][page_size][d_kv] of bf16, int8 or e4m3; k_scale, v_scale: f32
+ * [n_pages][n_kv_heads][page_size] for the 8-bit types (value = code * scale).  page_size a power of two in 16 .. 1024, d_kv 64 or 128,
+ * everything 16-byte aligned. */
+#define VLT5_KV_BF16 0
+#define VLT5_KV_INT8 1
+#define VLT5_KV_FP8 2
+typedef struct {
+    void *k, *v; float *k_scale, *v_scale;
+    int n_pages, n_kv_heads, d_kv, page_size, type;
+} vlt5_paged_kv;
+/* The sequences of a call.  Position p of sequence b is row p % page_size of page table[b][p / page_size]; a page id outside
+ * [0, n_pages) says that the page is not there: nothing is written to it, its keys are seen by nobody, it reads back as zeros.
+ * kv_lens[b]: keys of sequence b, the new tokens of the call INCLUDED (0 = none; at most max_pages * page_size count).  The new tokens of
+ * sequence b are rows cu_q[b] .. cu_q[b + 1] - 1 of the token tensors and stand at its last positions; cu_q NULL: one token each,
+ * n_tok == B.  max_q: no sequence has more new tokens than this (0 = n_tok); tokens past it are not processed.  Rows of the token tensors
+ * behind cu_q[B] belong to nobody: they are neither read nor written.  All three arrays are i32 device memory, read by the kernels alone. */
+typedef struct {
+    const int *table, *kv_lens, *cu_q;
+    int B, max_pages, n_tok, max_q;
+} vlt5_paged_seqs;
+/* New keys | values (bf16, head h of a token at h * d_kv, token strides k_st / v_st) into the cache, quantised on the way: one scale per
+ * (token, head), the largest magnitude / 127 (int8) or / 448 (e4m3); a head of a token with an infinity or a NaN is stored as scale NaN.
+ * No two tokens of a call may share a row of the cache (two sequences whose tables share the page that both write to). */
+int vlt5_kv_page_write(const vlt5_paged_kv* c, const vlt5_paged_seqs* q, const void* k, long long k_st, const void* v, long long v_st, void* stream);
+/* ... and back: k_out, v_out bf16 [B][T][n_kv_heads * d_kv], positions 0 .. T-1 of every sequence, zeros at and past its length (cu_q and
+ * n_tok are not used): the layout vlt5_attn_fwd takes. */
+int vlt5_kv_page_read(const vlt5_paged_kv* c, const vlt5_paged_seqs* q, int T, void* k_out, void* v_out, void* stream);
+/* out = softmax(scale * q K^T + bias) V of the new tokens over the keys of their sequence (which are in the cache already: write first).
+ * q, out bf16 [n_tok] rows of H heads of d_kv, H a multiple of n_kv_heads (query head h reads kv head h / (H / n_kv_heads)).  causal: a token
+ * sees the positions up to its own, else all kv_lens[b].  rel_bias f32 [H][n_dist] (causal only): added to the score of a key that lies
+ * `dist` positions back, the last entry for every larger dist -- T5's bucketed bias of a decoder as a function of the distance.  A token
+ * that sees no key gets zeros and lse -inf.  lse (optional) f32 [n_tok][H].  max_kv: about the longest kv_lens (0 = the table's width); it
+ * only decides how the work is split.  workspace: vlt5_paged_attn_workspace_bytes of the same desc (0: none needed), 16-byte aligned, one
+ * per call in flight. */
+typedef struct {
+    vlt5_paged_kv kv; vlt5_paged_seqs seqs;
+    const void* q; long long q_st; void* out; long long o_st; float* lse;
+    const float* rel_bias; int n_dist;
+    int H; float scale; int causal, max_kv;
+    void* workspace; long long workspace_bytes;
+} vlt5_paged_attn_desc;
+long long vlt5_paged_attn_workspace_bytes(const vlt5_paged_attn_desc* d);
+int vlt5_paged_attn(const vlt5_paged_attn_desc* d, void* stream);
+
 int vlt5_decoder_bwd(const vlt5_config* c, const vlt5_step* s, void* stream);
 int vlt5_encoder_bwd(const vlt5_config* c, const vlt5_step* s, void* stream);
 

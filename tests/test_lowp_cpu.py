@@ -1,0 +1,116 @@
+"""CPU tests of the low-precision token-step's host side: descriptors mirror the header, the C entry points refuse what the kernels could
+not take before anything is launched, and the wrappers refuse tensors that are not on the GPU."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+import torch
+
+from conftest import ROOT
+
+ARG, ALIGN = 1001, 1002
+
+
+@pytest.fixture(scope="module")
+def built():
+    import __graft_entry__ as ge
+    ge.build()
+    from vqacl_amd import _lib
+    return _lib
+
+
+def test_struct_sizes_match_the_c_side(built, tmp_path):
+    names = {"vlt5_decode_linear_w4_desc": built.DecodeLinearW4Desc, "vlt5_paged_kv": built.PagedKV, "vlt5_paged_seqs": built.PagedSeqs,
+             "vlt5_paged_attn_desc": built.PagedAttnDesc}
+    src = tmp_path / "sz.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "vlt5_hip.h"\nint main(void){' + "".join(f'printf("%zu\\n", sizeof({n}));' for n in names)
+                   + 'printf("%zu %zu\\n", offsetof(vlt5_paged_attn_desc, scale), offsetof(vlt5_decode_linear_w4_desc, relu));return 0;}')
+    exe = tmp_path / "sz"
+    subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)])
+    got = subprocess.check_output([str(exe)], text=True).split()
+    assert [int(x) for x in got[:4]] == [C.sizeof(m) for m in names.values()]
+    assert [int(x) for x in got[4:]] == [built.PagedAttnDesc.scale.offset, built.DecodeLinearW4Desc.relu.offset]
+
+
+P = 4096            # a pointer that is never followed: every call below is refused on the host
+
+
+def test_w4_refusals(built):
+    f = built.lib().vlt5_decode_linear_w4
+    ok = dict(x_bf16=P, ldx=64, codes=P, scales=P, rows=1, N=8, K=64, group=32, out_bf16=P, ld_out_bf16=8)
+    assert f(None, None) == ARG
+    for change, rc in (({"x_bf16": None}, ARG), ({"codes": None}, ARG), ({"scales": None}, ARG), ({"out_bf16": None}, ARG), ({"rows": 0}, ARG), ({"rows": 257}, ARG),
+                       ({"N": 0}, ARG), ({"K": 0}, ARG), ({"group": 48}, ARG), ({"group": 256}, ARG), ({"ldx": 32}, ARG), ({"ld_out_bf16": 7}, ARG),
+                       ({"out_f32": P, "ld_out_f32": 4}, ARG), ({"resid": P, "ld_resid": 4}, ARG), ({"K": 48, "ldx": 48}, ALIGN), ({"ldx": 68}, ALIGN),
+                       ({"codes": P + 8}, ALIGN), ({"x_bf16": P + 2}, ALIGN)):
+        d = built.DecodeLinearW4Desc(**{**ok, **change})
+        assert f(C.byref(d), None) == rc, change
+    q = built.lib().vlt5_quant_w4
+    assert q(None, None, 64, 4, 64, 32, P, P, None) == ARG and q(P, P, 64, 4, 64, 32, P, P, None) == ARG and q(P, None, 64, 4, 64, 33, P, P, None) == ARG
+    assert q(P, None, 64, 0, 64, 32, P, P, None) == ARG and q(P, None, 32, 4, 64, 32, P, P, None) == ARG and q(P, None, 64, 4, 64, 32, None, P, None) == ARG
+    assert q(P, None, 64, 4, 40, 32, P, P, None) == ALIGN and q(P, None, 64, 4, 64, 32, P + 4, P, None) == ALIGN
+
+
+KV = dict(k=P, v=P, k_scale=P, v_scale=P, n_pages=4, n_kv_heads=2, d_kv=64, page_size=16, type=1)
+SEQ = dict(table=P, kv_lens=P, cu_q=None, B=2, max_pages=3, n_tok=2, max_q=1)
+BAD_KV = [({"k": None}, ARG), ({"v": None}, ARG), ({"k_scale": None}, ARG), ({"v_scale": None}, ARG), ({"n_pages": 0}, ARG), ({"n_kv_heads": 0}, ARG), ({"n_kv_heads": 2000}, ARG),
+          ({"d_kv": 96}, ARG), ({"d_kv": 32}, ARG), ({"page_size": 8}, ARG), ({"page_size": 48}, ARG), ({"page_size": 2048}, ARG), ({"type": 3}, ARG), ({"type": -1}, ARG),
+          ({"k": P + 8}, ALIGN), ({"v_scale": P + 4}, ALIGN)]
+BAD_SEQ = [({"table": None}, ARG), ({"kv_lens": None}, ARG), ({"B": 0}, ARG), ({"B": 65536}, ARG), ({"max_pages": 0}, ARG), ({"n_tok": -1}, ARG), ({"n_tok": 3}, ARG), ({"max_q": -1}, ARG)]
+
+
+def test_cache_refusals(built):
+    L = built.lib()
+    kv, seq = built.PagedKV(**KV), built.PagedSeqs(**SEQ)
+    for change, rc in BAD_KV:
+        bad = built.PagedKV(**{**KV, **change})
+        assert L.vlt5_kv_page_write(C.byref(bad), C.byref(seq), P, 128, P, 128, None) == rc, change
+        assert L.vlt5_kv_page_read(C.byref(bad), C.byref(seq), 4, P, P, None) == rc, change
+    for change, rc in BAD_SEQ:
+        bad = built.PagedSeqs(**{**SEQ, **change})
+        assert L.vlt5_kv_page_write(C.byref(kv), C.byref(bad), P, 128, P, 128, None) == rc, change
+        assert L.vlt5_kv_page_read(C.byref(kv), C.byref(bad), 4, P, P, None) == rc, change
+    w, r = L.vlt5_kv_page_write, L.vlt5_kv_page_read
+    a, s = C.byref(kv), C.byref(seq)
+    assert w(None, s, P, 128, P, 128, None) == ARG and w(a, None, P, 128, P, 128, None) == ARG and w(a, s, None, 128, P, 128, None) == ARG
+    assert w(a, s, P, 127, P, 128, None) == ARG and w(a, s, P, 132, P, 128, None) == ALIGN and w(a, s, P, 128, P + 2, 128, None) == ALIGN
+    assert r(a, s, -1, P, P, None) == ARG and r(a, s, 4, None, P, None) == ARG and r(a, s, 4, P, P + 8, None) == ALIGN
+    none = built.PagedSeqs(**{**SEQ, "n_tok": 0})
+    assert w(a, C.byref(none), P, 128, P, 128, None) == 0 and r(a, s, 0, P, P, None) == 0                # nothing to do: nothing is launched
+
+
+def test_attention_refusals(built):
+    L = built.lib()
+    ok = dict(q=P, q_st=256, out=P, o_st=256, H=4, scale=1.0, causal=1)
+
+    def desc(kv={}, seq={}, **change):
+        return built.PagedAttnDesc(kv=built.PagedKV(**{**KV, **kv}), seqs=built.PagedSeqs(**{**SEQ, **seq}), **{**ok, **change})
+    assert L.vlt5_paged_attn(None, None) == ARG and L.vlt5_paged_attn_workspace_bytes(None) == -1
+    for change, rc in BAD_KV:
+        assert L.vlt5_paged_attn(C.byref(desc(kv=change)), None) == rc, change
+        assert L.vlt5_paged_attn_workspace_bytes(C.byref(desc(kv=change))) == -1
+    for change, rc in BAD_SEQ:
+        assert L.vlt5_paged_attn(C.byref(desc(seq=change)), None) == rc, change
+    for change, rc in (({"q": None}, ARG), ({"out": None}, ARG), ({"H": 3}, ARG), ({"H": 0}, ARG), ({"q_st": 255}, ARG), ({"o_st": 128}, ARG), ({"rel_bias": P}, ARG),
+                       ({"rel_bias": P, "n_dist": 4, "causal": 0}, ARG), ({"q_st": 260}, ALIGN), ({"q": P + 2}, ALIGN), ({"out": P + 8}, ALIGN), ({"workspace": P + 4}, ALIGN)):
+        assert L.vlt5_paged_attn(C.byref(desc(**change)), None) == rc, change
+    # a long context of few sequences is shared out and needs a workspace of its own: too small is refused
+    long = dict(seq={"max_pages": 4096})
+    need = L.vlt5_paged_attn_workspace_bytes(C.byref(desc(**long)))
+    assert need > 0 and need % (2 * 4 * (64 + 2) * 4) == 0
+    assert L.vlt5_paged_attn(C.byref(desc(**long)), None) == ARG
+    assert L.vlt5_paged_attn(C.byref(desc(**long, workspace=P, workspace_bytes=need - 1)), None) == ARG
+    assert L.vlt5_paged_attn_workspace_bytes(C.byref(desc())) == 0
+    assert L.vlt5_paged_attn(C.byref(desc(seq={"n_tok": 0})), None) == 0
+
+
+def test_wrappers_refuse_host_tensors(built):
+    from vqacl_amd import ops
+    c = ops.KVPages(*(torch.zeros(2, 1, 16, 64, dtype=torch.int8) for _ in range(2)), *(torch.zeros(2, 1, 16) for _ in range(2)))
+    t, n, x = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32), torch.zeros(1, 64, dtype=torch.bfloat16)
+    w = ops.W4Weight(torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(8, 1, dtype=torch.bfloat16), 64)
+    for call in (lambda: ops.quant_w4(torch.zeros(4, 64)), lambda: ops.decode_linear_w4(x, w), lambda: ops.kv_page_write(c, x, x, t, n),
+                 lambda: ops.kv_page_read(c, t, n, 4), lambda: ops.paged_attn(x, c, t, n)):
+        with pytest.raises(built.Vlt5Error):
+            call()

@@ -175,6 +175,27 @@ class DecodeLinearDesc(C.Structure):
                 ("row_ssq", vp), ("n_row_ssq", c_i)]
 
 
+class DecodeLinearW4Desc(C.Structure):
+    _fields_ = [("x_bf16", vp), ("ldx", c_ll), ("codes", vp), ("scales", vp), ("rows", c_i), ("N", c_i), ("K", c_i), ("group", c_i),
+                ("alpha", c_f), ("out_bf16", vp), ("ld_out_bf16", c_ll), ("out_f32", vp), ("ld_out_f32", c_ll), ("resid", vp),
+                ("ld_resid", c_ll), ("relu", c_i)]
+
+
+class PagedKV(C.Structure):
+    _fields_ = [("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp), ("n_pages", c_i), ("n_kv_heads", c_i), ("d_kv", c_i),
+                ("page_size", c_i), ("type", c_i)]
+
+
+class PagedSeqs(C.Structure):
+    _fields_ = [("table", vp), ("kv_lens", vp), ("cu_q", vp), ("B", c_i), ("max_pages", c_i), ("n_tok", c_i), ("max_q", c_i)]
+
+
+class PagedAttnDesc(C.Structure):
+    _fields_ = [("kv", PagedKV), ("seqs", PagedSeqs), ("q", vp), ("q_st", c_ll), ("out", vp), ("o_st", c_ll), ("lse", vp),
+                ("rel_bias", vp), ("n_dist", c_i), ("H", c_i), ("scale", c_f), ("causal", c_i), ("max_kv", c_i), ("workspace", vp),
+                ("workspace_bytes", c_ll)]
+
+
 # name -> (restype, argtypes); every symbol declared in include/vlt5_hip.h
 PROTOTYPES = {
     "vlt5_abi_version": (c_i, []),
@@ -272,6 +293,12 @@ PROTOTYPES = {
     "vlt5_decode_linear_supported": (c_i, [c_i, c_i]),
     "vlt5_decode_linear_tiles": (c_i, [c_i, c_i, c_i, c_i]),
     "vlt5_decode_attn": (c_i, [C.POINTER(AttnDesc), vp]),
+    "vlt5_quant_w4": (c_i, [vp, vp, c_ll, c_i, c_i, c_i, vp, vp, vp]),
+    "vlt5_decode_linear_w4": (c_i, [C.POINTER(DecodeLinearW4Desc), vp]),
+    "vlt5_kv_page_write": (c_i, [C.POINTER(PagedKV), C.POINTER(PagedSeqs), vp, c_ll, vp, c_ll, vp]),
+    "vlt5_kv_page_read": (c_i, [C.POINTER(PagedKV), C.POINTER(PagedSeqs), c_i, vp, vp, vp]),
+    "vlt5_paged_attn_workspace_bytes": (c_ll, [C.POINTER(PagedAttnDesc)]),
+    "vlt5_paged_attn": (c_i, [C.POINTER(PagedAttnDesc), vp]),
     "vlt5_decoder_bwd": (c_i, [C.POINTER(Config), C.POINTER(Step), vp]),
     "vlt5_encoder_bwd": (c_i, [C.POINTER(Config), C.POINTER(Step), vp]),
 }

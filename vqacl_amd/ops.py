@@ -4,6 +4,7 @@ Every function enqueues on torch's current HIP stream.  Tensors must live on the
 on the host and nothing falls back to torch ops.
 """
 import ctypes as C
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -355,3 +356,196 @@ def enc_attn_sublayer_bwd(dy, sv, want_dscores=False):
     g.dy, g.dx, g.d_wqkv, g.d_wo, g.d_ln_w, g.d_scores = ptr(_need(dy, torch.float32)), ptr(dx), ptr(dwqkv), ptr(dwo), ptr(dln), ptr(ds)
     check(lib().vlt5_enc_attn_bwd(C.byref(e), C.byref(g), ptr(ws), stream_ptr()), "vlt5_enc_attn_bwd")
     return dx, dwqkv, dwo, dln, ds
+
+
+# ---- the token-step in low precision: 4-bit weights, a paged key/value cache, the attention over it -------------------------------
+FP8 = torch.float8_e4m3fn
+_KV_TYPE = {BF16: 0, torch.int8: 1, FP8: 2}
+
+
+class W4Weight(NamedTuple):
+    """A weight [N, K] in four bits: codes uint8 [N, K/2] (two e2m1 codes a byte, the even k in the low bits), scales bf16
+    [N, ceil(K/group)], one for `group` (32, 64 or 128) consecutive k.  Made by `quant_w4`."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    group: int
+
+
+class KVPages(NamedTuple):
+    """The paged key/value cache of one layer: k, v [pages, kv heads, page size, d_kv] (bf16, int8 or float8_e4m3fn) and, for the 8-bit
+    types, k_scale, v_scale f32 [pages, kv heads, page size].  Made by `kv_pages`."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
+
+
+def _here(dev):
+    """The raw current stream of the current device, which `dev` has to be (the library launches on the current device)."""
+    if dev.type != "cuda":
+        raise L.Vlt5Error("tensor must be on the GPU")
+    i = torch.cuda.current_device()
+    if dev.index != i:
+        raise L.Vlt5Error(f"tensor on {dev}, but cuda:{i} is the current device")
+    return torch._C._cuda_getCurrentRawStream(i)
+
+
+def _like(t, dev, dtype, shape, what):
+    """`t` is a contiguous tensor of this type and shape on `dev`."""
+    if t.device != dev or t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise L.Vlt5Error(f"{what}: expected a contiguous {dtype} tensor {tuple(shape)} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _rows(t, dev, cols, what):
+    """`t` is a 2-D bf16 tensor [rows, cols] on `dev` with unit column stride: (pointer, row stride)."""
+    if t.device != dev or t.dtype != BF16 or t.dim() != 2 or t.shape[1] != cols or (t.stride(1) != 1 and cols != 1):
+        raise L.Vlt5Error(f"{what}: expected bf16 rows of {cols} on {dev}, got {t.dtype} {tuple(t.shape)} with strides {tuple(t.stride())} on {t.device}")
+    st = t.stride(0)
+    return t.data_ptr(), st if t.shape[0] > 1 else max(st, (cols + 7) // 8 * 8)
+
+
+def quant_w4(w, group=128):
+    """A weight [N, K] (f32 or bf16, unit column stride, K a multiple of 32) as a `W4Weight`."""
+    st = _here(w.device)
+    if w.dim() != 2 or w.dtype not in (BF16, torch.float32) or w.stride(1) != 1 or group not in (32, 64, 128):
+        raise L.Vlt5Error(f"quant_w4: expected f32 or bf16 rows and group 32, 64 or 128, got {w.dtype} {tuple(w.shape)}, {group}")
+    N, K = w.shape
+    codes = torch.empty(N, K // 2, device=w.device, dtype=torch.uint8)
+    scales = torch.empty(N, -(-K // group), device=w.device, dtype=BF16)
+    f32 = w.dtype == torch.float32
+    check(lib().vlt5_quant_w4(w.data_ptr() if f32 else None, None if f32 else w.data_ptr(), max(w.stride(0), K) if N == 1 else w.stride(0), N, K, group,
+                              codes.data_ptr(), scales.data_ptr(), st), "vlt5_quant_w4")
+    return W4Weight(codes, scales, group)
+
+
+def decode_linear_w4(x, w, *, alpha=1.0, resid=None, relu=False, out_f32=False, out=None):
+    """act(alpha * x W^T (+ resid)) for a few rows x bf16 [rows <= 256, K] against a `W4Weight`; resid f32 [rows, N].  Returns bf16, or f32
+    with out_f32; `out` takes the result instead (its type decides; it may be `resid` itself)."""
+    dev = x.device
+    st = _here(dev)
+    N, K = w.codes.shape[0], w.codes.shape[1] * 2
+    codes = _like(w.codes, dev, torch.uint8, (N, K // 2), "codes")
+    scales = _like(w.scales, dev, BF16, (N, -(-K // w.group)), "scales")
+    xp, ldx = _rows(x, dev, K, "x")
+    rows = x.shape[0]
+    if out is None:
+        out = torch.empty(rows, N, device=dev, dtype=torch.float32 if out_f32 else BF16)
+    elif out.device != dev or out.dtype not in (BF16, torch.float32) or tuple(out.shape) != (rows, N) or out.stride(1) != 1:
+        raise L.Vlt5Error(f"out: expected bf16 or f32 rows [{rows}, {N}] on {dev}, got {out.dtype} {tuple(out.shape)} on {out.device}")
+    f32 = out.dtype == torch.float32
+    if resid is not None and (resid.device != dev or resid.dtype != torch.float32 or tuple(resid.shape) != (rows, N) or resid.stride(1) != 1):
+        raise L.Vlt5Error(f"resid: expected f32 rows [{rows}, {N}] on {dev}, got {resid.dtype} {tuple(resid.shape)} on {resid.device}")
+    if rows == 0:
+        return out
+    o, ldo = out.data_ptr(), max(out.stride(0), N) if rows == 1 else out.stride(0)
+    d = L.DecodeLinearW4Desc(xp, ldx, codes, scales, rows, N, K, w.group, alpha, None if f32 else o, ldo, o if f32 else None, ldo,
+                             None if resid is None else resid.data_ptr(), 0 if resid is None else (max(resid.stride(0), N) if rows == 1 else resid.stride(0)), relu)
+    check(lib().vlt5_decode_linear_w4(C.byref(d), st), "vlt5_decode_linear_w4")
+    return out
+
+
+def kv_pages(n_pages, n_kv_heads, d_kv, page_size=64, dtype=torch.int8, device="cuda"):
+    """An empty paged cache: bf16, int8 or float8_e4m3fn."""
+    if dtype not in _KV_TYPE:
+        raise L.Vlt5Error(f"kv_pages: bf16, int8 or float8_e4m3fn, got {dtype}")
+    shape = (n_pages, n_kv_heads, page_size, d_kv)
+    k, v = (torch.zeros(shape, device=device, dtype=torch.uint8 if dtype == FP8 else dtype).view(dtype) for _ in range(2))
+    if dtype == BF16:
+        return KVPages(k, v)
+    return KVPages(k, v, *(torch.zeros(shape[:3], device=device, dtype=torch.float32) for _ in range(2)))
+
+
+def _paged_kv(c, dev):
+    kind = _KV_TYPE.get(c.k.dtype)
+    if kind is None or c.k.dim() != 4:
+        raise L.Vlt5Error(f"cache: expected [pages, kv heads, page size, d_kv] of bf16, int8 or float8_e4m3fn, got {c.k.dtype} {tuple(c.k.shape)}")
+    n, h, page, d = shape = c.k.shape
+    k, v = _like(c.k, dev, c.k.dtype, shape, "cache.k"), _like(c.v, dev, c.k.dtype, shape, "cache.v")
+    ks = vs = None
+    if kind:
+        if c.k_scale is None or c.v_scale is None:
+            raise L.Vlt5Error("cache: an 8-bit cache needs its scales")
+        ks = _like(c.k_scale, dev, torch.float32, (n, h, page), "cache.k_scale")
+        vs = _like(c.v_scale, dev, torch.float32, (n, h, page), "cache.v_scale")
+    return L.PagedKV(k, v, ks, vs, n, h, d, page, kind)
+
+
+def _paged_seqs(table, kv_lens, cu_q, n_tok, max_q, dev):
+    if table.dim() != 2:
+        raise L.Vlt5Error(f"block table: expected [sequences, pages], got {tuple(table.shape)}")
+    B, mp = table.shape
+    t = _like(table, dev, torch.int32, (B, mp), "block table")
+    n = _like(kv_lens, dev, torch.int32, (B,), "kv_lens")
+    if cu_q is not None:
+        return L.PagedSeqs(t, n, _like(cu_q, dev, torch.int32, (B + 1,), "cu_q"), B, mp, n_tok, max_q or 0)
+    if n_tok not in (0, B):
+        raise L.Vlt5Error(f"{n_tok} tokens for {B} sequences: without cu_q every sequence has one")
+    return L.PagedSeqs(t, n, None, B, mp, n_tok, 1)
+
+
+def kv_page_write(cache, k, v, table, kv_lens, *, cu_q=None, max_q=None):
+    """New keys | values k, v bf16 [tokens, kv heads * d_kv] (any token stride) into the pages of their sequences, quantised on the way.
+
+    table i32 [B, pages of a sequence], kv_lens i32 [B]: keys of every sequence with the new tokens counted; cu_q i32 [B + 1]: first new
+    token of every sequence (None: one token each); max_q: the most new tokens any of them has.  A page id outside the cache = not there."""
+    dev = cache.k.device
+    st = _here(dev)
+    kv = _paged_kv(cache, dev)
+    kp, k_st = _rows(k, dev, kv.n_kv_heads * kv.d_kv, "k")
+    vp_, v_st = _rows(v, dev, kv.n_kv_heads * kv.d_kv, "v")
+    if k.shape != v.shape:
+        raise L.Vlt5Error(f"k and v differ: {tuple(k.shape)}, {tuple(v.shape)}")
+    s = _paged_seqs(table, kv_lens, cu_q, k.shape[0], max_q, dev)
+    if k.shape[0]:
+        check(lib().vlt5_kv_page_write(C.byref(kv), C.byref(s), kp, k_st, vp_, v_st, st), "vlt5_kv_page_write")
+
+
+def kv_page_read(cache, table, kv_lens, T):
+    """Positions 0 .. T-1 of every sequence back as (k, v) bf16 [B, T, kv heads * d_kv], zeros at and past its length: what `attn_fwd` takes."""
+    dev = cache.k.device
+    st = _here(dev)
+    kv = _paged_kv(cache, dev)
+    s = _paged_seqs(table, kv_lens, None, 0, None, dev)
+    k, v = (torch.empty(s.B, T, kv.n_kv_heads * kv.d_kv, device=dev, dtype=BF16) for _ in range(2))
+    check(lib().vlt5_kv_page_read(C.byref(kv), C.byref(s), T, k.data_ptr() if T else kv.k, v.data_ptr() if T else kv.v, st), "vlt5_kv_page_read")
+    return k, v
+
+
+def paged_attn(q, cache, table, kv_lens, *, cu_q=None, max_q=None, max_kv=None, scale=1.0, causal=True, rel_bias=None, out=None, want_lse=False):
+    """softmax(scale * q K^T + bias) V of the newest tokens, q bf16 [tokens, heads * d_kv] (any token stride), over the pages of their
+    sequences, whose keys are written already (table, kv_lens, cu_q, max_q as in `kv_page_write`).
+
+    heads: any multiple of the cache's; causal: a token sees the positions up to its own, else all keys; rel_bias f32 [heads, n]: added by
+    how far the key lies back, its last column for everything further (T5's decoder bias); max_kv: about the longest length, for the split
+    of the work only.  A token that sees no key gets zeros; rows of `out` that belong to no sequence keep what they hold.
+    Returns out bf16 [tokens, heads * d_kv], with want_lse also f32 [tokens, heads] (-inf without keys)."""
+    dev = q.device
+    st = _here(dev)
+    kv = _paged_kv(cache, dev)
+    if q.dim() != 2 or q.shape[1] % (kv.n_kv_heads * kv.d_kv) or not q.shape[1]:
+        raise L.Vlt5Error(f"q: expected rows of a multiple of {kv.n_kv_heads} heads of {kv.d_kv}, got {tuple(q.shape)}")
+    n, width = q.shape
+    H = width // kv.d_kv
+    qp, q_st = _rows(q, dev, width, "q")
+    s = _paged_seqs(table, kv_lens, cu_q, n, max_q, dev)
+    if out is None:
+        out = torch.empty(n, width, device=dev, dtype=BF16)
+    op, o_st = _rows(out, dev, width, "out")
+    if out.shape[0] != n:
+        raise L.Vlt5Error(f"out: expected {n} rows, got {out.shape[0]}")
+    lse = torch.empty(n, H, device=dev, dtype=torch.float32) if want_lse else None
+    bias, nd = None, 0
+    if rel_bias is not None:
+        if not causal or rel_bias.dim() != 2 or rel_bias.shape[1] < 1:
+            raise L.Vlt5Error(f"rel_bias: f32 [heads, distances] of a causal call, got {tuple(rel_bias.shape)}, causal={causal}")
+        nd = rel_bias.shape[1]
+        bias = _like(rel_bias, dev, torch.float32, (H, nd), "rel_bias")
+    if n:
+        d = L.PagedAttnDesc(kv, s, qp, q_st, op, o_st, None if lse is None else lse.data_ptr(), bias, nd, H, scale, causal, max_kv or 0, None, 0)
+        need = lib().vlt5_paged_attn_workspace_bytes(C.byref(d))
+        if need > 0:
+            ws = torch.empty(need, device=dev, dtype=torch.uint8)
+            d.workspace, d.workspace_bytes = ws.data_ptr(), need
+        check(lib().vlt5_paged_attn(C.byref(d), st), "vlt5_paged_attn")
+    return (out, lse) if want_lse else out
