@@ -80,108 +80,164 @@ struct W4Args {
     int relu;
 };
 
-// A workgroup owns 16 * NT columns and 16 * MT rows; its waves share the reduction in chunks of 128 k and meet in LDS.  The rows of x are the
-// A operand, the weights the B operand, so that a lane's four sums belong to ONE column and one scale serves them.  A reduction may be
-// taken in any order as long as both operands agree, so the k that a lane's dword stands for follows the group length: the 32 k of one
-// matrix instruction must lie in one group, whose sum is scaled in f32 and added to the total.
-template <int G, int MT, int NT>
-__global__ __launch_bounds__(512) void w4_kernel(const W4Args a) {
-    extern __shared__ __attribute__((aligned(16))) float4 w4_red[];            // [waves][MT][NT][64]
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, NW = blockDim.x >> 6;
-    const int r16 = lane & 15, kq = lane >> 4;
-    const int n_tile = blockIdx.x * (16 * NT), m_tile = blockIdx.y * (16 * MT);
-    constexpr int GPC = 128 / G;                                               // groups per chunk
-    constexpr int DW = 4 / GPC;                                                // dwords of a lane per group
-    f32x4_t tot[MT][NT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) tot[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    const int chunks = (a.K + 127) / 128;
-    for (int c = w; c < chunks; c += NW) {
-        uint32_t cw[NT][4];
-        float sc[NT][GPC];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            int n = n_tile + j * 16 + r16;
-            n = n < a.N ? n : a.N - 1;                                         // columns past the end repeat the last one, never stored
-            const unsigned char* row = a.codes + (size_t)n * (a.K / 2);
-#pragma unroll
-            for (int gi = 0; gi < GPC; ++gi) {
-                const int k = c * 128 + gi * G + kq * (8 * DW);
-#pragma unroll
-                for (int e = 0; e < DW; ++e) cw[j][gi * DW + e] = k + e * 8 < a.K ? *reinterpret_cast<const uint32_t*>(row + (k + e * 8) / 2) : 0u;
-                sc[j][gi] = c * GPC + gi < a.groups ? bf16_to_f32(a.scales[(size_t)n * a.groups + c * GPC + gi]) : 0.f;
-            }
-        }
-        f32x4_t acc[MT][NT];
-#pragma unroll
-        for (int gi = 0; gi < GPC; ++gi) {
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int e = 0; e < DW; ++e) {
-                const int k = c * 128 + gi * G + kq * (8 * DW) + e * 8;
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    const int m = m_tile + i * 16 + r16;
-                    bf16x8_t fx = {0, 0, 0, 0, 0, 0, 0, 0};
-                    if (m < a.rows && k < a.K) fx = *reinterpret_cast<const bf16x8_t*>(a.x + (size_t)m * a.ldx + k);
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx, fp4x8(cw[j][gi * DW + e]), acc[i][j], 0, 0, 0);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) tot[i][j][r] = fmaf(sc[j][gi], acc[i][j][r], tot[i][j][r]);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) w4_red[((w * MT + i) * NT + j) * 64 + lane] = make_float4(tot[i][j][0], tot[i][j][1], tot[i][j][2], tot[i][j][3]);
-    __syncthreads();
-    for (int t = w; t < MT * NT; t += NW) {
-        const int i = t / NT, j = t % NT;
-        float4 v = w4_red[t * 64 + lane];
-        for (int ww = 1; ww < NW; ++ww) {
-            const float4 o = w4_red[(ww * MT * NT + t) * 64 + lane];
-            v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-        }
-        const int n = n_tile + j * 16 + r16;
-        const float s[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int m = m_tile + i * 16 + kq * 4 + r;
-            if (m >= a.rows || n >= a.N) continue;
-            float y = s[r] * a.alpha;
-            if (a.resid) y += a.resid[(size_t)m * a.ldr + n];
-            if (a.relu) y = y > 0.f ? y : (y != y ? y : 0.f);
-            if (a.out_f) a.out_f[(size_t)m * a.ldf + n] = y;
-            if (a.out_b) a.out_b[(size_t)m * a.ldo + n] = f32_to_bf16(y);
-        }
-    }
+__device__ __forceinline__ void w4_store(const W4Args& a, int m, int n, float sum) {
+    if (m >= a.rows || n >= a.N) return;
+    float y = sum * a.alpha;
+    if (a.resid) y += a.resid[(size_t)m * a.ldr + n];
+    if (a.relu) y = y > 0.f ? y : (y != y ? y : 0.f);
+    if (a.out_f) a.out_f[(size_t)m * a.ldf + n] = y;
+    if (a.out_b) a.out_b[(size_t)m * a.ldo + n] = f32_to_bf16(y);
 }
 
-template <int G, int MT, int NT>
-int w4_launch(const W4Args& a, hipStream_t st) {
+// A workgroup owns 16 rows and 8 / KW tiles of 16 columns; each tile's reduction is shared by KW waves in runs of neighbouring chunks of 128 k,
+// whose sums meet in LDS in the order of the waves.  The rows of x are the A operand, the weights the B operand, so that a lane's four sums
+// belong to ONE column and one scale serves them.  A reduction may be taken in any order as long as both operands agree, so the k that a lane
+// holds follows the group length: the 32 k of one matrix instruction lie in one group, whose sum is scaled in f32 and added to the total.
+//
+// What bounds it at these sizes is not memory but the address unit: a load whose neighbouring lanes lie in different rows (the operand's own
+// layout) costs 64 accesses instead of 16.  So nothing is loaded in operand layout: x goes to LDS once per workgroup in whole lines (row stride
+// KS + 8 values: the sixteen rows of an operand start in sixteen bank groups), a chunk of codes (16 columns x 64 bytes) is loaded with four
+// neighbouring lanes per column and turned round through one KB of LDS of the wave, and the scales of four chunks come with one load, one
+// chunk per lane group.  Rows of x longer than LDS are taken in slabs of KS.  Against loads in operand layout (us per call in a replayed graph):
+// 16 x 32200 x 768 11.1 -> 6.0, 1 x 4096 x 14336 11.0 -> 9.0 (29 MB: 5.4 TB/s less 3.3 us of launch), 200 x 5000 x 1024 22.2 -> 11.6; two or
+// four row tiles per workgroup, sixteen waves, and a ring of more than four chunks were all slower.
+template <int G, int KW>
+__global__ __launch_bounds__(512) void w4_kernel(const W4Args a, int KS) {
+    extern __shared__ __attribute__((aligned(16))) char w4_smem[];
+    constexpr int GPC = 128 / G, DW = G / 32;                                  // groups per chunk, dwords of a lane per group
+    constexpr int TW = 8 / KW, U = 4;                                          // column tiles; chunks requested ahead
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, kq = lane >> 4;
+    const int kw = w % KW;
+    const int n_tile = (blockIdx.x * TW + w / KW) * 16, m_tile = blockIdx.y * 16;
+    const int rows = min(16, a.rows - m_tile);
+    char* turn = w4_smem + w * 1024;
+    bf16_t* xs = reinterpret_cast<bf16_t*>(w4_smem + 8 * 1024);
+    const int ld = KS + 8;
+    // loads: lane l has piece (l & 3) of column l >> 2; LDS slot l, pieces swapped within the column so that the operand reads spread over the banks
+    const int lcol = lane >> 2, lseg = (lane & 3) ^ ((lane >> 4) & 3);
+    const unsigned char* wrow = a.codes + (size_t)min(n_tile + lcol, a.N - 1) * (a.K / 2);      // columns past the end repeat the last one, never stored
+    const bf16_t* srow = a.scales + (size_t)min(n_tile + r16, a.N - 1) * a.groups;
+    const bf16_t* xl = xs + min(r16, rows - 1) * ld;
+    auto load_w = [&](int c) {                                                 // (a piece past the end of the row: any codes, x is zero there)
+        return *reinterpret_cast<const uint4*>(wrow + c * 64 + (c * 128 + lseg * 32 < a.K ? lseg * 16 : 0));
+    };
+    struct Scales { bf16_t v[GPC]; };
+    auto load_s = [&](int c, int end) {                                        // of chunk c + kq
+        Scales s;
+        const int at = min(c + kq, end - 1) * GPC;
+        if (at + GPC <= a.groups) {
+            __builtin_memcpy(&s, srow + at, sizeof s);
+        } else {
+#pragma unroll
+            for (int i = 0; i < GPC; ++i) s.v[i] = srow[min(at + i, a.groups - 1)];
+        }
+        return s;
+    };
+    f32x4_t tot = {0.f, 0.f, 0.f, 0.f};
     const int chunks = (a.K + 127) / 128;
-    const int NW = chunks >= 8 ? 8 : chunks;
-    const dim3 grid((a.N + 16 * NT - 1) / (16 * NT), (a.rows + 16 * MT - 1) / (16 * MT));
-    hipLaunchKernelGGL((w4_kernel<G, MT, NT>), grid, dim3(64 * NW), (size_t)NW * MT * NT * 1024, st, a);
+    for (int cs = 0; cs < chunks; cs += KS / 128) {
+        const int cnt = min(KS / 128, chunks - cs);
+        const int c0 = cs + cnt * kw / KW, c1 = cs + cnt * (kw + 1) / KW;
+        uint4 wr[U];
+        Scales sn;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (c0 + u < c1) wr[u] = load_w(c0 + u);                           // on their way while x is staged
+        if (c0 < c1) sn = load_s(c0, c1);
+        if (cs) __syncthreads();                                               // every wave is done with the slab before
+        const int kmax = min(KS, a.K - cs * 128), pieces = (cnt * 128) / 8;
+        for (int i0 = threadIdx.x; i0 < rows * pieces; i0 += 4 * 512) {
+            uint4 v[4];
+            int at[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int i = i0 + q * 512, r = i / pieces, k = (i - r * pieces) * 8;
+                v[q] = make_uint4(0, 0, 0, 0);
+                at[q] = i < rows * pieces ? r * ld + k : -1;
+                if (at[q] >= 0 && k < kmax) v[q] = *reinterpret_cast<const uint4*>(a.x + (size_t)(m_tile + r) * a.ldx + cs * 128 + k);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (at[q] >= 0) *reinterpret_cast<uint4*>(xs + at[q]) = v[q];
+        }
+        __syncthreads();
+        for (int c = c0; c < c1; c += U) {
+            const Scales sc = sn;
+            if (c + U < c1) sn = load_s(c + U, c1);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (c + u >= c1) break;
+                __builtin_amdgcn_wave_barrier();                               // (LDS operations of one wave complete in order: only the compiler has to keep it)
+                *reinterpret_cast<uint4*>(turn + lane * 16) = wr[u];
+                __builtin_amdgcn_wave_barrier();
+                if (c + u + U < c1) wr[u] = load_w(c + u + U);
+                uint32_t sp[(GPC + 1) / 2];
+                __builtin_memcpy(sp, &sc, sizeof sc);
+#pragma unroll
+                for (int i = 0; i < (GPC + 1) / 2; ++i) sp[i] = __builtin_amdgcn_ds_bpermute((u * 16 + r16) * 4, sp[i]);
+#pragma unroll
+                for (int gi = 0; gi < GPC; ++gi) {
+                    // this lane's codes of the group: 4 * DW bytes at gi * G / 2 + kq * 4 * DW of the column's 64
+                    const int byte = gi * (G / 2) + kq * (4 * DW);
+                    const char* p = turn + r16 * 64 + (((byte >> 4) ^ (r16 >> 2)) << 4) + (byte & 15);
+                    uint32_t cw[DW];
+                    __builtin_memcpy(cw, __builtin_assume_aligned(p, 4 * DW), sizeof cw);
+                    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int e = 0; e < DW; ++e) {
+                        const bf16x8_t fx = *reinterpret_cast<const bf16x8_t*>(xl + (c + u - cs) * 128 + gi * G + kq * (8 * DW) + e * 8);
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx, fp4x8(cw[e]), acc, 0, 0, 0);
+                    }
+                    const float s = __uint_as_float(gi & 1 ? sp[gi / 2] & 0xffff0000u : sp[gi / 2] << 16);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) tot[r] = fmaf(s, acc[r], tot[r]);
+                }
+            }
+        }
+    }
+    if constexpr (KW > 1) {
+        __syncthreads();                                                       // codes and x are read no more: the sums take their place
+        float4* red = reinterpret_cast<float4*>(w4_smem);
+        red[w * 64 + lane] = make_float4(tot[0], tot[1], tot[2], tot[3]);
+        __syncthreads();
+        if (kw) return;
+#pragma unroll
+        for (int q = 1; q < KW; ++q) {
+            const float4 o = red[(w + q) * 64 + lane];
+            tot[0] += o.x; tot[1] += o.y; tot[2] += o.z; tot[3] += o.w;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) w4_store(a, m_tile + kq * 4 + r, n_tile + r16, tot[r]);
+}
+
+template <int G, int KW>
+int w4_launch(const W4Args& a, hipStream_t st) {
+    static std::atomic<unsigned long long> done{0};
+    const int rows = a.rows < 16 ? a.rows : 16;
+    const int kpad = (a.K + 127) & ~127, room = 148 * 1024 / 2 / rows - 8;      // 8 KB of the 160 are for the codes on their way
+    const int KS = kpad <= room ? kpad : room & ~127;
+    const int rc = vlt5_lds_optin((const void*)w4_kernel<G, KW>, 160 * 1024, done);
+    if (rc) return rc;
+    const dim3 grid(((a.N + 15) / 16 + 8 / KW - 1) / (8 / KW), (a.rows + 15) / 16);
+    hipLaunchKernelGGL((w4_kernel<G, KW>), grid, dim3(512), 8 * 1024 + rows * (KS + 8) * 2, st, a, KS);
     LAUNCH_CHECK();
     return VLT5_OK;
 }
+// The shares of a reduction: as many as leave no more than one workgroup per CU (256), since what a workgroup stages is then read once per CU;
+// never more than there are chunks.  Measured: 3 x 14336 x 4096 in 1 / 2 / 4 / 8 shares 15.7 / 11.6 / 11.3 / 13.9 us (rule: 2), 5 x 4097 x 14336
+// 39.6 / 25.7 / 16.6 / 21.6 (rule: 4; with 8 the 257th workgroup runs alone), 80 x 2304 x 768 5.3 / 4.8 / 5.2 / 5.7 (2), 1 x 768 x 768
+// 4.9 / 4.2 / 3.8 / 3.5 (8), 16 x 32200 x 768 6.0 / 7.1 / 9.3 / 13.3 (1).
 template <int G>
-int w4_rows(const W4Args& a, hipStream_t st) {
-    if (a.rows <= 16) return w4_launch<G, 1, 1>(a, st);
-    if (a.rows <= 32) return w4_launch<G, 2, 1>(a, st);
-    return w4_launch<G, 4, 1>(a, st);
+int w4_shares(const W4Args& a, hipStream_t st) {
+    const long long tiles = (a.N + 15) / 16, blocks = (a.rows + 15) / 16;
+    const int chunks = (a.K + 127) / 128;
+    int kw = 8;
+    while (kw > 1 && ((tiles * kw + 7) / 8 * blocks > 256 || kw / 2 >= chunks)) kw /= 2;
+    if (kw == 8) return w4_launch<G, 8>(a, st);
+    if (kw == 4) return w4_launch<G, 4>(a, st);
+    if (kw == 2) return w4_launch<G, 2>(a, st);
+    return w4_launch<G, 1>(a, st);
 }
 
 }  // namespace
@@ -205,7 +261,7 @@ extern "C" int vlt5_quant_w4(const float* w_f32, const void* w_bf16, long long l
 
 extern "C" int vlt5_decode_linear_w4(const vlt5_decode_linear_w4_desc* d, void* stream) {
     if (!d || !d->x_bf16 || !d->codes || !d->scales || (!d->out_bf16 && !d->out_f32)) return VLT5_ERR_ARG;
-    if (d->rows <= 0 || d->rows > VLT5_W4_MAX_ROWS || d->N <= 0 || d->K <= 0 || d->ldx < d->K) return VLT5_ERR_ARG;
+    if (d->rows <= 0 || d->rows > VLT5_W4_MAX_ROWS || d->N <= 0 || d->N > 1 << 28 || d->K <= 0 || d->K > 1 << 28 || d->ldx < d->K) return VLT5_ERR_ARG;
     if (d->group != 32 && d->group != 64 && d->group != 128) return VLT5_ERR_ARG;
     if ((d->out_bf16 && d->ld_out_bf16 < d->N) || (d->out_f32 && d->ld_out_f32 < d->N) || (d->resid && d->ld_resid < d->N)) return VLT5_ERR_ARG;
     if ((d->K & 31) || (d->ldx & 7) || (((uintptr_t)d->x_bf16 | (uintptr_t)d->codes) & 15)) return VLT5_ERR_ALIGN;
@@ -216,7 +272,7 @@ extern "C" int vlt5_decode_linear_w4(const vlt5_decode_linear_w4_desc* d, void* 
     a.out_b = (bf16_t*)d->out_bf16; a.ldo = d->ld_out_bf16; a.out_f = d->out_f32; a.ldf = d->ld_out_f32;
     a.resid = d->resid; a.ldr = d->ld_resid; a.relu = d->relu;
     hipStream_t st = (hipStream_t)stream;
-    if (d->group == 32) return w4_rows<32>(a, st);
-    if (d->group == 64) return w4_rows<64>(a, st);
-    return w4_rows<128>(a, st);
+    if (d->group == 32) return w4_shares<32>(a, st);
+    if (d->group == 64) return w4_shares<64>(a, st);
+    return w4_shares<128>(a, st);
 }

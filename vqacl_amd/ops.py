@@ -384,64 +384,80 @@ def _here(dev):
     """The raw current stream of the current device, which `dev` has to be (the library launches on the current device)."""
     if dev.type != "cuda":
         raise L.Vlt5Error("tensor must be on the GPU")
-    i = torch.cuda.current_device()
+    i = torch._C._cuda_getDevice()
     if dev.index != i:
         raise L.Vlt5Error(f"tensor on {dev}, but cuda:{i} is the current device")
     return torch._C._cuda_getCurrentRawStream(i)
 
 
-def _like(t, dev, dtype, shape, what):
-    """`t` is a contiguous tensor of this type and shape on `dev`."""
-    if t.device != dev or t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise L.Vlt5Error(f"{what}: expected a contiguous {dtype} tensor {tuple(shape)} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+def _refuse(dev, *want):
+    """Raises for the first (name, tensor, dtypes, shape, contiguous) that is not so: what a call's one combined check found to be wrong."""
+    for name, t, dtypes, shape, contiguous in want:
+        if t is None:
+            raise L.Vlt5Error(f"{name} is missing")
+        got = f"got {t.dtype} {tuple(t.shape)} with strides {tuple(t.stride())} on {t.device}"
+        if t.device != dev or t.dtype not in dtypes or t.dim() != len(shape) or any(s is not None and s != n for s, n in zip(shape, t.shape)):
+            raise L.Vlt5Error(f"{name}: expected {' or '.join(map(str, dtypes))} {shape} on {dev}, {got}")
+        if not t.is_contiguous() if contiguous else t.stride(-1) != 1 and t.shape[-1] > 1:
+            raise L.Vlt5Error(f"{name}: expected {'a contiguous tensor' if contiguous else 'unit column stride'}, {got}")
+    raise L.Vlt5Error("sizes do not fit together: " + ", ".join(f"{n} {tuple(t.shape)}" for n, t, *_ in want))
 
 
-def _rows(t, dev, cols, what):
-    """`t` is a 2-D bf16 tensor [rows, cols] on `dev` with unit column stride: (pointer, row stride)."""
-    if t.device != dev or t.dtype != BF16 or t.dim() != 2 or t.shape[1] != cols or (t.stride(1) != 1 and cols != 1):
-        raise L.Vlt5Error(f"{what}: expected bf16 rows of {cols} on {dev}, got {t.dtype} {tuple(t.shape)} with strides {tuple(t.stride())} on {t.device}")
-    st = t.stride(0)
-    return t.data_ptr(), st if t.shape[0] > 1 else max(st, (cols + 7) // 8 * 8)
+def _row_stride(t, rows, cols):
+    """Row stride of a 2-D tensor; that of a single row, which torch leaves arbitrary, is made up."""
+    return t.stride(0) if rows > 1 else (cols + 7) // 8 * 8
 
 
 def quant_w4(w, group=128):
     """A weight [N, K] (f32 or bf16, unit column stride, K a multiple of 32) as a `W4Weight`."""
-    st = _here(w.device)
-    if w.dim() != 2 or w.dtype not in (BF16, torch.float32) or w.stride(1) != 1 or group not in (32, 64, 128):
-        raise L.Vlt5Error(f"quant_w4: expected f32 or bf16 rows and group 32, 64 or 128, got {w.dtype} {tuple(w.shape)}, {group}")
+    dev = w.device
+    st = _here(dev)
+    if w.dim() != 2 or w.dtype not in (BF16, torch.float32) or w.stride(1) != 1:
+        _refuse(dev, ("w", w, (BF16, torch.float32), (None, None), False))
     N, K = w.shape
-    codes = torch.empty(N, K // 2, device=w.device, dtype=torch.uint8)
-    scales = torch.empty(N, -(-K // group), device=w.device, dtype=BF16)
+    if group not in (32, 64, 128):
+        raise L.Vlt5Error(f"group: 32, 64 or 128, got {group}")
+    codes = torch.empty(N, K // 2, device=dev, dtype=torch.uint8)
+    scales = torch.empty(N, -(-K // group), device=dev, dtype=BF16)
     f32 = w.dtype == torch.float32
-    check(lib().vlt5_quant_w4(w.data_ptr() if f32 else None, None if f32 else w.data_ptr(), max(w.stride(0), K) if N == 1 else w.stride(0), N, K, group,
-                              codes.data_ptr(), scales.data_ptr(), st), "vlt5_quant_w4")
+    check(lib().vlt5_quant_w4(w.data_ptr() if f32 else None, None if f32 else w.data_ptr(), _row_stride(w, N, K), N, K, group, codes.data_ptr(),
+                              scales.data_ptr(), st), "vlt5_quant_w4")
     return W4Weight(codes, scales, group)
 
 
 def decode_linear_w4(x, w, *, alpha=1.0, resid=None, relu=False, out_f32=False, out=None):
     """act(alpha * x W^T (+ resid)) for a few rows x bf16 [rows <= 256, K] against a `W4Weight`; resid f32 [rows, N].  Returns bf16, or f32
     with out_f32; `out` takes the result instead (its type decides; it may be `resid` itself)."""
+    codes, scales, group = w
     dev = x.device
     st = _here(dev)
-    N, K = w.codes.shape[0], w.codes.shape[1] * 2
-    codes = _like(w.codes, dev, torch.uint8, (N, K // 2), "codes")
-    scales = _like(w.scales, dev, BF16, (N, -(-K // w.group)), "scales")
-    xp, ldx = _rows(x, dev, K, "x")
-    rows = x.shape[0]
+    if group not in (32, 64, 128):
+        raise L.Vlt5Error(f"group: 32, 64 or 128, got {group}")
+    if x.dim() != 2 or codes.dim() != 2:
+        _refuse(dev, ("x", x, (BF16,), (None, None), False), ("codes", codes, (torch.uint8,), (None, None), True))
+    (rows, K), (N, K2) = x.shape, codes.shape
+    groups = -(-K // group)
+    if (x.dtype is not BF16 or x.stride(1) != 1 or K != 2 * K2 or codes.dtype is not torch.uint8 or codes.device != dev or not codes.is_contiguous()
+            or scales.dtype is not BF16 or scales.device != dev or scales.shape != (N, groups) or not scales.is_contiguous()):
+        _refuse(dev, ("x", x, (BF16,), (None, 2 * K2), False), ("codes", codes, (torch.uint8,), (N, K2), True), ("scales", scales, (BF16,), (N, groups), True))
     if out is None:
         out = torch.empty(rows, N, device=dev, dtype=torch.float32 if out_f32 else BF16)
-    elif out.device != dev or out.dtype not in (BF16, torch.float32) or tuple(out.shape) != (rows, N) or out.stride(1) != 1:
-        raise L.Vlt5Error(f"out: expected bf16 or f32 rows [{rows}, {N}] on {dev}, got {out.dtype} {tuple(out.shape)} on {out.device}")
-    f32 = out.dtype == torch.float32
-    if resid is not None and (resid.device != dev or resid.dtype != torch.float32 or tuple(resid.shape) != (rows, N) or resid.stride(1) != 1):
-        raise L.Vlt5Error(f"resid: expected f32 rows [{rows}, {N}] on {dev}, got {resid.dtype} {tuple(resid.shape)} on {resid.device}")
-    if rows == 0:
-        return out
-    o, ldo = out.data_ptr(), max(out.stride(0), N) if rows == 1 else out.stride(0)
-    d = L.DecodeLinearW4Desc(xp, ldx, codes, scales, rows, N, K, w.group, alpha, None if f32 else o, ldo, o if f32 else None, ldo,
-                             None if resid is None else resid.data_ptr(), 0 if resid is None else (max(resid.stride(0), N) if rows == 1 else resid.stride(0)), relu)
-    check(lib().vlt5_decode_linear_w4(C.byref(d), st), "vlt5_decode_linear_w4")
+        f32, ldo = out_f32, N
+    else:
+        f32 = out.dtype is torch.float32
+        if not (f32 or out.dtype is BF16) or out.shape != (rows, N) or out.device != dev or (N > 1 and out.stride(1) != 1):
+            _refuse(dev, ("out", out, (BF16, torch.float32), (rows, N), False))
+        ldo = out.stride(0) if rows > 1 else N
+    rp, ldr = None, 0
+    if resid is not None:
+        if resid.dtype is not torch.float32 or resid.shape != (rows, N) or resid.device != dev or (N > 1 and resid.stride(1) != 1):
+            _refuse(dev, ("resid", resid, (torch.float32,), (rows, N), False))
+        rp, ldr = resid.data_ptr(), resid.stride(0) if rows > 1 else N
+    if rows:
+        o = out.data_ptr()
+        d = L.DecodeLinearW4Desc(x.data_ptr(), _row_stride(x, rows, K), codes.data_ptr(), scales.data_ptr(), rows, N, K, group, alpha, None if f32 else o, ldo,
+                                 o if f32 else None, ldo, rp, ldr, relu)
+        check(lib().vlt5_decode_linear_w4(C.byref(d), st), "vlt5_decode_linear_w4")
     return out
 
 
@@ -456,32 +472,38 @@ def kv_pages(n_pages, n_kv_heads, d_kv, page_size=64, dtype=torch.int8, device="
     return KVPages(k, v, *(torch.zeros(shape[:3], device=device, dtype=torch.float32) for _ in range(2)))
 
 
-def _paged_kv(c, dev):
-    kind = _KV_TYPE.get(c.k.dtype)
-    if kind is None or c.k.dim() != 4:
-        raise L.Vlt5Error(f"cache: expected [pages, kv heads, page size, d_kv] of bf16, int8 or float8_e4m3fn, got {c.k.dtype} {tuple(c.k.shape)}")
-    n, h, page, d = shape = c.k.shape
-    k, v = _like(c.k, dev, c.k.dtype, shape, "cache.k"), _like(c.v, dev, c.k.dtype, shape, "cache.v")
-    ks = vs = None
-    if kind:
-        if c.k_scale is None or c.v_scale is None:
-            raise L.Vlt5Error("cache: an 8-bit cache needs its scales")
-        ks = _like(c.k_scale, dev, torch.float32, (n, h, page), "cache.k_scale")
-        vs = _like(c.v_scale, dev, torch.float32, (n, h, page), "cache.v_scale")
-    return L.PagedKV(k, v, ks, vs, n, h, d, page, kind)
-
-
-def _paged_seqs(table, kv_lens, cu_q, n_tok, max_q, dev):
-    if table.dim() != 2:
-        raise L.Vlt5Error(f"block table: expected [sequences, pages], got {tuple(table.shape)}")
+def _paged(cache, table, kv_lens, cu_q, n_tok, max_q, dev):
+    """The cache and the sequences of a call as the library takes them."""
+    k, v, ks, vs = cache
+    kind = _KV_TYPE.get(k.dtype)
+    if kind is None or k.dim() != 4 or table.dim() != 2:
+        _refuse(dev, ("cache.k", k, tuple(_KV_TYPE), (None,) * 4, True), ("block table", table, (torch.int32,), (None, None), True))
+    shape = k.shape
     B, mp = table.shape
-    t = _like(table, dev, torch.int32, (B, mp), "block table")
-    n = _like(kv_lens, dev, torch.int32, (B,), "kv_lens")
-    if cu_q is not None:
-        return L.PagedSeqs(t, n, _like(cu_q, dev, torch.int32, (B + 1,), "cu_q"), B, mp, n_tok, max_q or 0)
-    if n_tok not in (0, B):
-        raise L.Vlt5Error(f"{n_tok} tokens for {B} sequences: without cu_q every sequence has one")
-    return L.PagedSeqs(t, n, None, B, mp, n_tok, 1)
+    if v.dtype is not k.dtype or v.shape != shape or v.device != dev or not k.is_contiguous() or not v.is_contiguous():
+        _refuse(dev, ("cache.k", k, (k.dtype,), tuple(shape), True), ("cache.v", v, (k.dtype,), tuple(shape), True))
+    n, h, page, d = shape
+    ksp = vsp = None
+    if kind:
+        rows = (n, h, page)
+        if (ks is None or vs is None or ks.dtype is not torch.float32 or vs.dtype is not torch.float32 or ks.shape != rows or vs.shape != rows or ks.device != dev
+                or vs.device != dev or not ks.is_contiguous() or not vs.is_contiguous()):
+            _refuse(dev, ("cache.k_scale", ks, (torch.float32,), rows, True), ("cache.v_scale", vs, (torch.float32,), rows, True))
+        ksp, vsp = ks.data_ptr(), vs.data_ptr()
+    if (table.dtype is not torch.int32 or table.device != dev or not table.is_contiguous() or kv_lens.dtype is not torch.int32 or kv_lens.device != dev
+            or kv_lens.shape != (B,) or not kv_lens.is_contiguous()):
+        _refuse(dev, ("block table", table, (torch.int32,), (B, mp), True), ("kv_lens", kv_lens, (torch.int32,), (B,), True))
+    cu = None
+    if cu_q is None:
+        max_q = 1
+        if n_tok != B and n_tok:
+            raise L.Vlt5Error(f"{n_tok} tokens for {B} sequences: without cu_q every sequence has one")
+    else:
+        if cu_q.dtype is not torch.int32 or cu_q.device != dev or cu_q.shape != (B + 1,) or not cu_q.is_contiguous():
+            _refuse(dev, ("cu_q", cu_q, (torch.int32,), (B + 1,), True))
+        cu = cu_q.data_ptr()
+    return (L.PagedKV(k.data_ptr(), v.data_ptr(), ksp, vsp, n, h, d, page, kind), L.PagedSeqs(table.data_ptr(), kv_lens.data_ptr(), cu, B, mp, n_tok, max_q or 0),
+            h, d, B)
 
 
 def kv_page_write(cache, k, v, table, kv_lens, *, cu_q=None, max_q=None):
@@ -489,26 +511,27 @@ def kv_page_write(cache, k, v, table, kv_lens, *, cu_q=None, max_q=None):
 
     table i32 [B, pages of a sequence], kv_lens i32 [B]: keys of every sequence with the new tokens counted; cu_q i32 [B + 1]: first new
     token of every sequence (None: one token each); max_q: the most new tokens any of them has.  A page id outside the cache = not there."""
-    dev = cache.k.device
+    dev = k.device
     st = _here(dev)
-    kv = _paged_kv(cache, dev)
-    kp, k_st = _rows(k, dev, kv.n_kv_heads * kv.d_kv, "k")
-    vp_, v_st = _rows(v, dev, kv.n_kv_heads * kv.d_kv, "v")
-    if k.shape != v.shape:
-        raise L.Vlt5Error(f"k and v differ: {tuple(k.shape)}, {tuple(v.shape)}")
-    s = _paged_seqs(table, kv_lens, cu_q, k.shape[0], max_q, dev)
-    if k.shape[0]:
-        check(lib().vlt5_kv_page_write(C.byref(kv), C.byref(s), kp, k_st, vp_, v_st, st), "vlt5_kv_page_write")
+    if k.dim() != 2 or cache.k.device != dev:
+        _refuse(dev, ("k", k, (BF16,), (None, None), False), ("cache.k", cache.k, tuple(_KV_TYPE), (None,) * 4, True))
+    n, width = k.shape
+    kv, seqs, h, d, _ = _paged(cache, table, kv_lens, cu_q, n, max_q, dev)
+    if k.dtype is not BF16 or v.dtype is not BF16 or width != h * d or v.shape != (n, width) or v.device != dev or k.stride(1) != 1 or v.stride(1) != 1:
+        _refuse(dev, ("k", k, (BF16,), (None, h * d), False), ("v", v, (BF16,), (n, h * d), False))
+    if n:
+        check(lib().vlt5_kv_page_write(C.byref(kv), C.byref(seqs), k.data_ptr(), _row_stride(k, n, width), v.data_ptr(), _row_stride(v, n, width), st), "vlt5_kv_page_write")
 
 
 def kv_page_read(cache, table, kv_lens, T):
     """Positions 0 .. T-1 of every sequence back as (k, v) bf16 [B, T, kv heads * d_kv], zeros at and past its length: what `attn_fwd` takes."""
     dev = cache.k.device
     st = _here(dev)
-    kv = _paged_kv(cache, dev)
-    s = _paged_seqs(table, kv_lens, None, 0, None, dev)
-    k, v = (torch.empty(s.B, T, kv.n_kv_heads * kv.d_kv, device=dev, dtype=BF16) for _ in range(2))
-    check(lib().vlt5_kv_page_read(C.byref(kv), C.byref(s), T, k.data_ptr() if T else kv.k, v.data_ptr() if T else kv.v, st), "vlt5_kv_page_read")
+    kv, seqs, h, d, B = _paged(cache, table, kv_lens, None, 0, None, dev)
+    k = torch.empty(B, T, h * d, device=dev, dtype=BF16)
+    v = torch.empty(B, T, h * d, device=dev, dtype=BF16)
+    if T:
+        check(lib().vlt5_kv_page_read(C.byref(kv), C.byref(seqs), T, k.data_ptr(), v.data_ptr(), st), "vlt5_kv_page_read")
     return k, v
 
 
@@ -522,30 +545,34 @@ def paged_attn(q, cache, table, kv_lens, *, cu_q=None, max_q=None, max_kv=None, 
     Returns out bf16 [tokens, heads * d_kv], with want_lse also f32 [tokens, heads] (-inf without keys)."""
     dev = q.device
     st = _here(dev)
-    kv = _paged_kv(cache, dev)
-    if q.dim() != 2 or q.shape[1] % (kv.n_kv_heads * kv.d_kv) or not q.shape[1]:
-        raise L.Vlt5Error(f"q: expected rows of a multiple of {kv.n_kv_heads} heads of {kv.d_kv}, got {tuple(q.shape)}")
+    if q.dim() != 2 or cache.k.device != dev:
+        _refuse(dev, ("q", q, (BF16,), (None, None), False), ("cache.k", cache.k, tuple(_KV_TYPE), (None,) * 4, True))
     n, width = q.shape
-    H = width // kv.d_kv
-    qp, q_st = _rows(q, dev, width, "q")
-    s = _paged_seqs(table, kv_lens, cu_q, n, max_q, dev)
+    kv, seqs, h, d, _ = _paged(cache, table, kv_lens, cu_q, n, max_q, dev)
+    if q.dtype is not BF16 or width % (h * d) or not width or q.stride(1) != 1:
+        raise L.Vlt5Error(f"q: expected bf16 rows of a multiple of {h} heads of {d}, got {q.dtype} {tuple(q.shape)} with strides {tuple(q.stride())}")
+    H = width // d
     if out is None:
-        out = torch.empty(n, width, device=dev, dtype=BF16)
-    op, o_st = _rows(out, dev, width, "out")
-    if out.shape[0] != n:
-        raise L.Vlt5Error(f"out: expected {n} rows, got {out.shape[0]}")
+        out, o_st = torch.empty(n, width, device=dev, dtype=BF16), width
+    else:
+        if out.dtype is not BF16 or out.shape != (n, width) or out.device != dev or out.stride(1) != 1:
+            _refuse(dev, ("out", out, (BF16,), (n, width), False))
+        o_st = _row_stride(out, n, width)
     lse = torch.empty(n, H, device=dev, dtype=torch.float32) if want_lse else None
     bias, nd = None, 0
     if rel_bias is not None:
-        if not causal or rel_bias.dim() != 2 or rel_bias.shape[1] < 1:
-            raise L.Vlt5Error(f"rel_bias: f32 [heads, distances] of a causal call, got {tuple(rel_bias.shape)}, causal={causal}")
-        nd = rel_bias.shape[1]
-        bias = _like(rel_bias, dev, torch.float32, (H, nd), "rel_bias")
+        if not causal or rel_bias.dim() != 2 or rel_bias.shape[0] != H or rel_bias.shape[1] < 1 or rel_bias.dtype is not torch.float32 or rel_bias.device != dev \
+                or not rel_bias.is_contiguous():
+            raise L.Vlt5Error(f"rel_bias: contiguous f32 [{H}, distances] of a causal call, got {rel_bias.dtype} {tuple(rel_bias.shape)} on {rel_bias.device}, causal={causal}")
+        bias, nd = rel_bias.data_ptr(), rel_bias.shape[1]
     if n:
-        d = L.PagedAttnDesc(kv, s, qp, q_st, op, o_st, None if lse is None else lse.data_ptr(), bias, nd, H, scale, causal, max_kv or 0, None, 0)
-        need = lib().vlt5_paged_attn_workspace_bytes(C.byref(d))
+        l = lib()
+        desc = L.PagedAttnDesc(kv, seqs, q.data_ptr(), _row_stride(q, n, width), out.data_ptr(), o_st, None if lse is None else lse.data_ptr(), bias, nd, H, scale,
+                               causal, max_kv or 0, None, 0)
+        ref = C.byref(desc)
+        need = l.vlt5_paged_attn_workspace_bytes(ref)
         if need > 0:
             ws = torch.empty(need, device=dev, dtype=torch.uint8)
-            d.workspace, d.workspace_bytes = ws.data_ptr(), need
-        check(lib().vlt5_paged_attn(C.byref(d), st), "vlt5_paged_attn")
+            desc.workspace, desc.workspace_bytes = ws.data_ptr(), need
+        check(l.vlt5_paged_attn(ref, st), "vlt5_paged_attn")
     return (out, lse) if want_lse else out
