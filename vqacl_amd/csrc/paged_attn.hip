@@ -10,6 +10,7 @@
 // 8-bit codes are exact in bf16; the scale of a key multiplies its score, the scale of a value its probability (in f32, before the one
 // rounding of the probabilities to bf16).
 #include "paged.h"
+#include <stdlib.h>
 
 namespace {
 
@@ -23,38 +24,13 @@ struct PagedAttnArgs {
     float scale;
     int causal;
     const float* bias; int nd;                // [H][nd] by distance, the last entry for everything further
-    int row_tiles, join_tiles, splits;
+    int row_tiles, splits;
     float* part_o; float* part_ml;            // [splits][n_tok * H][d_kv], [splits][n_tok * H][2]
 };
 
 constexpr float LOG2E = 1.4426950408889634f;
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// one lane's four consecutive dwords / pairs of a row of codes as MFMA operands
-template <int T, int DK>
-__device__ __forceinline__ void load_key_frags(const unsigned char* row, int kq, bf16x8_t (&f)[DK / 32]) {
-    if constexpr (T == VLT5_KV_BF16) {
-#pragma unroll
-        for (int i = 0; i < DK / 32; ++i) f[i] = *reinterpret_cast<const bf16x8_t*>(row + (i * 32 + kq * 8) * 2);
-    } else {
-#pragma unroll
-        for (int c = 0; c < DK / 64; ++c) {
-            const uint4 u = *reinterpret_cast<const uint4*>(row + c * 64 + kq * 16);
-            const uint2 a = codes_to_bf16<T>(u.x), b = codes_to_bf16<T>(u.y), e = codes_to_bf16<T>(u.z), d = codes_to_bf16<T>(u.w);
-            f[c * 2] = __builtin_bit_cast(bf16x8_t, make_uint4(a.x, a.y, b.x, b.y));
-            f[c * 2 + 1] = __builtin_bit_cast(bf16x8_t, make_uint4(e.x, e.y, d.x, d.y));
-        }
-    }
-}
-// ... and the query row in the same order of d
-template <int T, int DK>
-__device__ __forceinline__ void load_query_frags(const bf16_t* row, int kq, bf16x8_t (&f)[DK / 32]) {
-#pragma unroll
-    for (int i = 0; i < DK / 32; ++i) {
-        const int d = T == VLT5_KV_BF16 ? i * 32 + kq * 8 : (i >> 1) * 64 + kq * 16 + (i & 1) * 8;
-        f[i] = *reinterpret_cast<const bf16x8_t*>(row + d);
-    }
-}
 // DK / 16 neighbouring values of a row of V, raw
 template <int T, int DK> struct VRow { uint32_t w[DK / 16 * KvType<T>::BYTES / 4]; };
 template <int T, int DK>
@@ -79,10 +55,38 @@ __device__ __forceinline__ uint32_t vpair(const VRow<T, DK>& a, const VRow<T, DK
     }
 }
 
+// The raw rows of 32 keys, as one lane holds them: for the scores keys 16 i + lane % 16 (16-byte pieces of the row), for the output the rows
+// 16 i + 4 * (lane / 16) + 0 .. 3, DK / 16 values of each.
+template <int T, int DK>
+struct KeyStep {
+    static constexpr int KP = DK * KvType<T>::BYTES / 64;
+    vlt5_u32x4_t k[2][KP];
+    VRow<T, DK> v[2][4];
+    float4 ks[2], vs[2];
+    __device__ __forceinline__ void load(const PagedAttnArgs& a, int hk, const int (&page)[2], int t, int r16, int kq) {
+        constexpr int ROWB = DK * KvType<T>::BYTES;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const size_t base = (((size_t)max(page[i], 0) * a.Hkv + hk) << a.s.page_shift) + ((t + i * 16) & ((1 << a.s.page_shift) - 1));
+            const unsigned char* kp = a.k + (base + r16) * ROWB + kq * 16;
+#pragma unroll
+            for (int c = 0; c < KP; ++c) k[i][c] = *reinterpret_cast<const vlt5_u32x4_t*>(kp + c * 64);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][e] = load_vrow<T, DK>(a.v + (base + kq * 4 + e) * ROWB + r16 * (ROWB / 16));
+            if constexpr (KvType<T>::SCALED) {
+                ks[i] = *reinterpret_cast<const float4*>(a.ks + base + kq * 4);
+                vs[i] = *reinterpret_cast<const float4*>(a.vs + base + kq * 4);
+            }
+        }
+    }
+};
+
+// NW waves share the keys of a row tile in steps of 32, the next step's rows on their way while one is used; the page ids of a wave's next 32
+// steps come with one load, two to a step.
 template <int T, int DK, int NW>
-__global__ __launch_bounds__(NW * 64) void paged_attn_kernel(const PagedAttnArgs a) {
-    constexpr int NF = DK / 32, ND = DK / 16, ROWB = DK * KvType<T>::BYTES;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, kq = lane >> 4;
+__global__ __launch_bounds__(NW * 64, 2) void paged_attn_kernel(const PagedAttnArgs a) {
+    constexpr int NF = DK / 32, ND = DK / 16;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, kq = lane >> 4;
     int id = blockIdx.x;
     const int sp = id % a.splits; id /= a.splits;
     const int rt = id % a.row_tiles; id /= a.row_tiles;
@@ -92,105 +96,153 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_kernel(const PagedAttnArgs
     if (rt * 16 >= rows) return;
     const int r = min(rt * 16 + r16, rows - 1);
     const int tok = r / a.g, hq = hk * a.g + r % a.g;
-    const int pos = sq.len - sq.nq + tok;                                          // this row's position (negative: more new tokens than keys)
+    const int p0 = sq.len - sq.nq, pos = p0 + tok;                                 // this row's position (negative: more new tokens than keys)
     const int L = a.causal ? min(pos + 1, sq.len) : sq.len;                       // keys this row sees
-    const int first = sq.len - sq.nq + rt * 16 / a.g, last = sq.len - sq.nq + min(rt * 16 + 15, rows - 1) / a.g;
+    const int first = p0 + rt * 16 / a.g, last = p0 + min(rt * 16 + 15, rows - 1) / a.g;
     const int Lmin = a.causal ? first + 1 : sq.len, Lmax = max(a.causal ? last + 1 : sq.len, 0);
-    const int per = ((Lmax + a.splits - 1) / a.splits + 63) & ~63;
+    const int per = ((Lmax + a.splits - 1) / a.splits + 32 * NW - 1) / (32 * NW) * (32 * NW);
     const int lo = min(sp * per, Lmax), hi = min(lo + per, Lmax);
 
+    // d in the order of the keys' 16-byte pieces
     bf16x8_t fq[NF];
-    load_query_frags<T, DK>(a.q + (size_t)(sq.q0 + tok) * a.q_st + hq * DK, kq, fq);
+    const bf16_t* qrow = a.q + (size_t)(sq.q0 + tok) * a.q_st + hq * DK;
+#pragma unroll
+    for (int i = 0; i < NF; ++i) fq[i] = *reinterpret_cast<const bf16x8_t*>(qrow + (T == VLT5_KV_BF16 ? i * 32 + kq * 8 : (i >> 1) * 64 + kq * 16 + (i & 1) * 8));
     const float* bias = a.bias ? a.bias + (size_t)hq * a.nd : nullptr;
+    const float bias_far = bias ? bias[a.nd - 1] : 0.f;
+    const float unit = bias ? 1.f : LOG2E, rest = bias ? LOG2E : 1.f;              // without a bias scores are kept in powers of two
+    const float cs = a.scale * unit;
 
     f32x4_t o[ND];
 #pragma unroll
     for (int j = 0; j < ND; ++j) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
-    for (int t0 = lo + w * 64; t0 < hi; t0 += NW * 64) {
-        size_t base[4];
-        bool there[4];
+    const int steps = hi > lo ? (hi - lo + 31) / 32 : 0, mine = steps > w ? (steps - w + NW - 1) / NW : 0;
+    auto at = [&](int i) { return lo + (i * NW + w) * 32; };
+    int ids = -1;                                                                  // lane j: page of the 16 keys j & 1 of step (i & ~31) + j / 2
+    auto load_ids = [&](int i) {
+        const int t = at(i + (lane >> 1)) + (lane & 1) * 16;
+        ids = i + (lane >> 1) < mine && t < hi ? paged_page(a.s, b, t) : -1;
+    };
+    int pg[2][2];
+    KeyStep<T, DK> st[2];
+    auto load = [&](int i, int buf) {
+        pg[buf][0] = __builtin_amdgcn_readlane(ids, (i & 31) * 2);
+        pg[buf][1] = __builtin_amdgcn_readlane(ids, (i & 31) * 2 + 1);
+        st[buf].load(a, hk, pg[buf], at(i), r16, kq);
+    };
+    auto use = [&](int i, int buf) {
+        KeyStep<T, DK>& x = st[buf];
+        const int t0 = at(i);
+        f32x4_t sc[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int pg = t0 + i * 16 < hi ? paged_page(a.s, b, t0 + i * 16) : -1;
-            there[i] = pg >= 0;
-            base[i] = (((size_t)max(pg, 0) * a.Hkv + hk) << a.s.page_shift) + ((t0 + i * 16) & ((1 << a.s.page_shift) - 1));
-        }
-        const bool whole = t0 + 64 <= min(Lmin, hi) && there[0] && there[1] && there[2] && there[3];
-        VRow<T, DK> vr[4][4];
-        float4 kscale[4], vscale[4];
-        f32x4_t sc[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            bf16x8_t fk[NF];
-            load_key_frags<T, DK>(a.k + (base[i] + r16) * ROWB, kq, fk);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) vr[i][e] = load_vrow<T, DK>(a.v + (base[i] + kq * 4 + e) * ROWB + r16 * (ROWB / 16));
-            kscale[i] = vscale[i] = make_float4(1.f, 1.f, 1.f, 1.f);
-            if constexpr (KvType<T>::SCALED) {
-                kscale[i] = *reinterpret_cast<const float4*>(a.ks + base[i] + kq * 4);
-                vscale[i] = *reinterpret_cast<const float4*>(a.vs + base[i] + kq * 4);
-            }
+        for (int i = 0; i < 2; ++i) {
             sc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int f = 0; f < NF; ++f) sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fk[f], fq[f], sc[i], 0, 0, 0);
-        }
-        float p[4][4], top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float kk[4] = {kscale[i].x, kscale[i].y, kscale[i].z, kscale[i].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int t = t0 + i * 16 + kq * 4 + e;
-                float s = sc[i][e] * (kk[e] * a.scale);
-                if (bias) s += bias[min(max(pos - t, 0), a.nd - 1)];
-                if (!whole) s = there[i] && t < L ? s : -INFINITY;
-                p[i][e] = s;
-                top = fmaxf(top, s);
+            for (int f = 0; f < NF; ++f) {
+                bf16x8_t fk;
+                if constexpr (T == VLT5_KV_BF16) fk = __builtin_bit_cast(bf16x8_t, x.k[i][f]);
+                else {
+                    const uint2 c0 = codes_to_bf16<T>(x.k[i][f >> 1][(f & 1) * 2]), c1 = codes_to_bf16<T>(x.k[i][f >> 1][(f & 1) * 2 + 1]);
+                    fk = __builtin_bit_cast(bf16x8_t, make_uint4(c0.x, c0.y, c1.x, c1.y));
+                }
+                sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fk, fq[f], sc[i], 0, 0, 0);
             }
         }
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float mn = fmaxf(m, top), ms = mn == -INFINITY ? 0.f : mn;            // a row that has seen no key yet stays at -inf, sum 0
-        const float fix = exp2_hw((m - ms) * LOG2E);
-        m = mn;
-        l *= fix;
+        const bool whole = t0 + 32 <= min(Lmin, hi) && pg[buf][0] >= 0 && pg[buf][1] >= 0;
+        float p[2][4], top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < ND; ++j)
+        for (int i = 0; i < 2; ++i) {
+            float kk[4] = {1.f, 1.f, 1.f, 1.f};
+            if constexpr (KvType<T>::SCALED) { kk[0] = x.ks[i].x; kk[1] = x.ks[i].y; kk[2] = x.ks[i].z; kk[3] = x.ks[i].w; }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[j][e] *= fix;
-        uint32_t pb[4][2];
+            for (int e = 0; e < 4; ++e) p[i][e] = sc[i][e] * (kk[e] * cs);
+        }
+        if (bias) {
+            if (first - (t0 + 31) >= a.nd - 1) {                                   // every key further than the table reaches
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float vv[4] = {vscale[i].x, vscale[i].y, vscale[i].z, vscale[i].w};
-            float x[4];
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[i][e] += bias_far;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[i][e] += bias[min(max(pos - (t0 + i * 16 + kq * 4 + e), 0), a.nd - 1)];
+            }
+        }
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[i][e] = pg[buf][i] >= 0 && t0 + i * 16 + kq * 4 + e < L ? p[i][e] : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, p[i][e]);
+        // the running maximum moves only when a new one is more than 2^8 away: until then probabilities up to 256 do no harm (f32 sums, bf16
+        // relative to the value), and neither the exchange between the row's four lanes nor the rescaling is needed
+        if (__any(top > m + 8.f * (unit / LOG2E))) {
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float mn = fmaxf(m, top), ms = mn == -INFINITY ? 0.f : mn;        // a row that has seen no key yet stays at -inf, sum 0
+            const float fix = exp2_hw((m - ms) * rest);
+            m = mn;
+            l *= fix;
+#pragma unroll
+            for (int j = 0; j < ND; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[j][e] *= fix;
+        }
+        const float ms = m == -INFINITY ? 0.f : m;
+        uint32_t pb[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float vv[4] = {1.f, 1.f, 1.f, 1.f}, y[4];
+            if constexpr (KvType<T>::SCALED) { vv[0] = x.vs[i].x; vv[1] = x.vs[i].y; vv[2] = x.vs[i].z; vv[3] = x.vs[i].w; }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float pe = exp2_hw((p[i][e] - ms) * LOG2E);
+                const float pe = exp2_hw((p[i][e] - ms) * rest);
                 l += pe;
-                x[e] = pe * vv[e];
-                if (!whole) {                                                        // what lies behind the last key may hold anything, NaN too
-                    const bool in = there[i] && t0 + i * 16 + kq * 4 + e < sq.len;
-                    if (!(in && t0 + i * 16 + kq * 4 + e < L)) x[e] = 0.f;
-                    if (!in) vr[i][e] = VRow<T, DK>{};
+                y[e] = pe * vv[e];
+            }
+            if (!whole) {                                                          // what lies behind the last key may hold anything, NaN too
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int t = t0 + i * 16 + kq * 4 + e;
+                    const bool in = pg[buf][i] >= 0 && t < sq.len;
+                    if (!(in && t < L)) y[e] = 0.f;
+                    if (!in) x.v[i][e] = VRow<T, DK>{};
                 }
             }
-            pb[i][0] = pack_bf16x2(x[0], x[1]);
-            pb[i][1] = pack_bf16x2(x[2], x[3]);
+            pb[i][0] = pack_bf16x2(y[0], y[1]);
+            pb[i][1] = pack_bf16x2(y[2], y[3]);
         }
+        const bf16x8_t fp = __builtin_bit_cast(bf16x8_t, make_uint4(pb[0][0], pb[0][1], pb[1][0], pb[1][1]));
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const bf16x8_t fp = __builtin_bit_cast(bf16x8_t, make_uint4(pb[2 * h][0], pb[2 * h][1], pb[2 * h + 1][0], pb[2 * h + 1][1]));
-#pragma unroll
-            for (int j = 0; j < ND; ++j) {
-                const uint4 fv = make_uint4(vpair<T, DK>(vr[2 * h][0], vr[2 * h][1], j), vpair<T, DK>(vr[2 * h][2], vr[2 * h][3], j),
-                                            vpair<T, DK>(vr[2 * h + 1][0], vr[2 * h + 1][1], j), vpair<T, DK>(vr[2 * h + 1][2], vr[2 * h + 1][3], j));
-                o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, fv), fp, o[j], 0, 0, 0);
-            }
+        for (int j = 0; j < ND; ++j) {
+            const uint4 fv = make_uint4(vpair<T, DK>(x.v[0][0], x.v[0][1], j), vpair<T, DK>(x.v[0][2], x.v[0][3], j), vpair<T, DK>(x.v[1][0], x.v[1][1], j),
+                                        vpair<T, DK>(x.v[1][2], x.v[1][3], j));
+            o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, fv), fp, o[j], 0, 0, 0);
         }
+    };
+    if (mine) {
+        load_ids(0);
+        load(0, 0);
+    }
+    for (int i = 0; i < mine; i += 2) {
+        if (i + 1 < mine) load(i + 1, 1);                                          // (i is even: never the first of 32 steps)
+        use(i, 0);
+        if (i + 2 < mine) {
+            if (((i + 2) & 31) == 0) load_ids(i + 2);
+            load(i + 2, 0);
+        }
+        if (i + 1 < mine) use(i + 1, 1);
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
+    m = bias ? m : m / LOG2E;
 
     // ---- the waves' shares of the keys meet in LDS, always in the order of the waves ----
     __shared__ float so[NW][16][DK + 4];
@@ -273,6 +325,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
 #pragma unroll
     for (int i = 0; i < NKS; ++i) fq[i] = *reinterpret_cast<const bf16x8_t*>(qrow + i * 16 + h * 8);
     const float* bias = BIAS ? a.bias + (size_t)hq * a.nd : nullptr;
+    const float bias_far = BIAS ? bias[a.nd - 1] : 0.f;
     const float unit = BIAS ? 1.f : LOG2E;                                              // without a bias scores are kept in powers of two
     const float cs = a.scale * unit;
 
@@ -280,20 +333,27 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
     vlt5_u32x4_t kr[KP];
     uint32_t vr[8][VW];
     float scl = 0.f;
-    // rows of a 16-key group are in one page; `row` = first cache row of the group, or -1
-    auto group_row = [&](int t) -> long long {
-        const int pg = t < hi ? paged_page(a.s, b, t) : -1;
-        return pg < 0 ? -1 : (long long)((((size_t)pg * a.Hkv + hk) << a.s.page_shift) + (t & ((1 << a.s.page_shift) - 1)));
+    // the keys of 16 are in one page; lane j: page of the j-th 16 keys of the 16 tiles from (tile & ~15) on, or -1
+    int ids = -1, pg[4], pn[4];                                                         // ... and those of this tile and the next
+    const int tiles = (hi - lo + 63) / 64;
+    auto load_ids = [&](int tile) {
+        const int t = lo + tile * 64 + lane * 16;
+        ids = t < hi ? paged_page(a.s, b, t) : -1;
     };
-    auto fetch = [&](int t0) {
+    auto first_row = [&](int page, int t) { return (((size_t)max(page, 0) * a.Hkv + hk) << a.s.page_shift) + (t & ((1 << a.s.page_shift) - 1)); };
+    auto fetch = [&](int tile) {
+        const int t0 = lo + tile * 64;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pn[i] = __builtin_amdgcn_readlane(ids, (tile & 15) * 4 + i);
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
-            const int key = __builtin_amdgcn_readfirstlane((i * 256 + w * 64) / KCH) + lane / KCH;      // 64 / KCH keys a wave: 4 .. 16
-            const long long g0 = group_row(t0 + __builtin_amdgcn_readfirstlane((i * 256 + w * 64) / KCH / 16 * 16));
-            kr[i] = *reinterpret_cast<const vlt5_u32x4_t*>(a.k + (size_t)(max(g0, 0LL) + (key & 15)) * ROWB + (lane % KCH) * 16);
+            // the pieces of 64 lanes are 64 / KCH (4, 8 or 16) keys of one group of 16
+            const int base = (i * 256 + w * 64) / KCH, grp = base >> 4;
+            const int page = grp == 0 ? pn[0] : (grp == 1 ? pn[1] : (grp == 2 ? pn[2] : pn[3]));
+            kr[i] = *reinterpret_cast<const vlt5_u32x4_t*>(a.k + (first_row(page, t0 + grp * 16) + ((base & 15) + lane / KCH)) * ROWB + (lane % KCH) * 16);
         }
-        const long long g0 = group_row(t0 + w * 16);
-        const unsigned char* vp = a.v + (size_t)max(g0, 0LL) * ROWB + r32 * (NT * BY);
+        const int g0 = w == 0 ? pn[0] : (w == 1 ? pn[1] : (w == 2 ? pn[2] : pn[3]));
+        const unsigned char* vp = a.v + first_row(g0, t0 + w * 16) * ROWB + r32 * (NT * BY);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const unsigned char* p = vp + (size_t)((e >> 2) * 8 + h * 4 + (e & 3)) * ROWB;
@@ -303,10 +363,9 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
         }
         if constexpr (KvType<T>::SCALED) {
             if (w < 2) {                                                                // wave 0: key scales, wave 1: value scales
-                const int pg = t0 + lane < hi ? paged_page(a.s, b, t0 + lane) : -1;
-                const size_t at = (((size_t)max(pg, 0) * a.Hkv + hk) << a.s.page_shift) + ((t0 + lane) & ((1 << a.s.page_shift) - 1));
-                scl = (w ? a.vs : a.ks)[at];
-                if (w && (pg < 0 || t0 + lane >= sq.len)) scl = 0.f;
+                const int page = lane < 16 ? pn[0] : (lane < 32 ? pn[1] : (lane < 48 ? pn[2] : pn[3]));
+                scl = (w ? a.vs : a.ks)[first_row(page, t0 + lane)];
+                if (w && (page < 0 || t0 + lane >= sq.len)) scl = 0.f;
             }
         }
         // what lies behind the last key or in a page that is not there may hold anything, NaN too
@@ -353,16 +412,22 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[j][e] = 0.f;
     float m = -INFINITY, l = 0.f;
-    if (lo < hi) {
-        fetch(lo);
+    if (tiles > 0) {
+        load_ids(0);
+        fetch(0);
         stage(smem);
     }
     __syncthreads();
-    int cur = 0;
-    for (int t0 = lo; t0 < hi; t0 += 64, cur ^= 1) {
+    for (int tile = 0; tile < tiles; ++tile) {
+        const int t0 = lo + tile * 64, cur = tile & 1;
         const char* buf = smem + cur * BUF;
-        const bool more = t0 + 64 < hi;
-        if (more) fetch(t0 + 64);
+        const bool more = tile + 1 < tiles;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pg[i] = pn[i];
+        if (more) {
+            if (((tile + 1) & 15) == 0) load_ids(tile + 1);
+            fetch(tile + 1);
+        }
         if (t0 < wLmax) {
             f32x16_t s[2];
 #pragma unroll
@@ -374,12 +439,9 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
                     s[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(buf + (i * 32 + r32) * KROW + (k * 16 + h * 8) * 2), fq[k], s[i], 0, 0, 0);
             }
             // register e of tile i: key t0 + i * 32 + 8 * (e / 4) + 4 * h + e % 4
-            bool there = true;
-            if (t0 + 64 > wLmin) there = false;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) there = there && group_row(t0 + i * 16) >= 0;
+            const bool whole = t0 + 64 <= wLmin && min(min(pg[0], pg[1]), min(pg[2], pg[3])) >= 0;
+            const bool far = BIAS && p0 + min(wr0, rows - 1) / a.g - (t0 + 63) >= a.nd - 1;      // every key further than the table reaches
             const float* ks = reinterpret_cast<const float*>(buf + KBYTES + VBYTES);
-            float c = cs;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -389,18 +451,28 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
                     const float kk[4] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float v = s[i][q * 4 + e] * (KvType<T>::SCALED ? kk[e] * c : c);
-                        const int t = t0 + i * 32 + q * 8 + h * 4 + e;
-                        if constexpr (BIAS) v += bias[min(max(pos - t, 0), a.nd - 1)];
-                        s[i][q * 4 + e] = v;
+                        s[i][q * 4 + e] *= KvType<T>::SCALED ? kk[e] * cs : cs;
                     }
                 }
-            if (!there) {
+            if constexpr (BIAS) {
+                if (far) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s[i][e] += bias_far;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s[i][e] += bias[min(max(pos - (t0 + i * 32 + e / 4 * 8 + h * 4 + e % 4), 0), a.nd - 1)];
+                }
+            }
+            if (!whole) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        const bool page = group_row(t0 + i * 32 + q / 2 * 16) >= 0;
+                        const bool page = pg[i * 2 + q / 2] >= 0;
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             s[i][q * 4 + e] = page && t0 + i * 32 + q * 8 + h * 4 + e < L ? s[i][q * 4 + e] : -INFINITY;
@@ -486,38 +558,53 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
     }
 }
 
-// joins the splits of a row, in their order
-template <int DK>
+// Joins the splits of a row: lane j has the maximum and sum of split j (there are at most 64), its weight goes to all lanes by v_readlane, and
+// every split's output is requested without waiting for the one before.  WPR waves share the splits of a row (4 where there are many: a few
+// rows of a long context would otherwise be one chain of 64 loads), and meet in LDS in their order.
+template <int DK, int WPR>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) {
-    int id = blockIdx.x;
-    const int rt = id % a.join_tiles; id /= a.join_tiles;
-    const int hk = id % a.Hkv, b = id / a.Hkv;
+    constexpr int VEC = DK / 64;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = w % WPR;
+    const int per = a.s.max_q * a.g;                                               // rows of a pair that may exist
+    const long long row_id = (long long)blockIdx.x * (4 / WPR) + w / WPR;
+    const int pair = (int)(row_id / per), rr = (int)(row_id % per);
+    const int hk = pair % a.Hkv, b = pair / a.Hkv;
+    if (b >= a.s.B) return;                                                        // (WPR = 4: the whole workgroup)
     const PagedSeq sq = paged_seq(a.s, b);
-    const int rows = min(sq.nq, a.s.max_q) * a.g;
-    for (int i = threadIdx.x; i < 16 * (DK / 4); i += 256) {
-        const int rr = rt * 16 + i / (DK / 4), d = i % (DK / 4) * 4;
-        if (rr >= rows) continue;
-        const size_t row = (size_t)(sq.q0 + rr / a.g) * a.H + hk * a.g + rr % a.g;
-        const size_t step = (size_t)a.s.n_tok * a.H;
-        float mx = -INFINITY;
-        for (int sp = 0; sp < a.splits; ++sp) mx = fmaxf(mx, a.part_ml[(sp * step + row) * 2]);
-        const float ms = mx == -INFINITY ? 0.f : mx;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float sum = 0.f;
-        for (int sp = 0; sp < a.splits; ++sp) {
-            const float f = exp2_hw((a.part_ml[(sp * step + row) * 2] - ms) * LOG2E);
-            const float4 x = *reinterpret_cast<const float4*>(a.part_o + (sp * step + row) * DK + d);
-            sum += a.part_ml[(sp * step + row) * 2 + 1] * f;
-            acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
-        }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        *reinterpret_cast<uint2*>(a.out + (row / a.H) * a.o_st + (row % a.H) * DK + d) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-        if (a.lse && d == 0) a.lse[row] = sum == 0.f ? -INFINITY : mx + logf(sum);
+    if (rr >= min(sq.nq, a.s.max_q) * a.g) return;
+    const size_t row = (size_t)(sq.q0 + rr / a.g) * a.H + hk * a.g + rr % a.g, step = (size_t)a.s.n_tok * a.H;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < a.splits) ml = *reinterpret_cast<const float2*>(a.part_ml + (lane * step + row) * 2);
+    const int s0 = a.splits * part / WPR, s1 = a.splits * (part + 1) / WPR;
+    float acc[VEC] = {};
+    const float mx = wave_max(ml.x), ms = mx == -INFINITY ? 0.f : mx;
+    const float f = exp2_hw((ml.x - ms) * LOG2E);
+    const float sum = wave_sum(ml.y * f);
+#pragma unroll 8
+    for (int sp = s0; sp < s1; ++sp) {
+        const float* src = a.part_o + (sp * step + row) * DK + lane * VEC;
+        const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), sp));
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = fmaf(src[i], fs, acc[i]);
     }
+    if constexpr (WPR > 1) {
+        __shared__ float so[WPR][DK];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) so[part][lane * VEC + i] = acc[i];
+        __syncthreads();
+        if (part) return;
+#pragma unroll
+        for (int q = 1; q < WPR; ++q)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[i] += so[q][lane * VEC + i];
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    bf16_t* dst = a.out + (row / a.H) * a.o_st + (row % a.H) * DK + lane * VEC;
+    if constexpr (VEC == 2) *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+    else *dst = f32_to_bf16(acc[0] * inv);
+    if (a.lse && lane == 0) a.lse[row] = sum == 0.f ? -INFINITY : mx + logf(sum);
 }
 
-// The plan of a call, from what the host knows.  Up to 64 rows (tokens x heads of a group) go through the first kernel, more share their keys
-// through LDS.  Keys are shared out until the chip is full (1024 waves' worth of small workgroups, 512 large ones), no share below 512 keys.
 template <int T, int DK, bool BIAS>
 int chunk_launch(const PagedAttnArgs& a, unsigned blocks, hipStream_t st) {
     static std::atomic<unsigned long long> done{0};
@@ -527,7 +614,7 @@ int chunk_launch(const PagedAttnArgs& a, unsigned blocks, hipStream_t st) {
     hipLaunchKernelGGL((paged_chunk_kernel<T, DK, BIAS>), dim3(blocks), dim3(256), bytes, st, a);
     return VLT5_OK;
 }
-struct PagedPlan { int chunk, row_tiles, splits; };
+struct PagedPlan { int chunk, row_tiles, splits, waves; };
 PagedPlan paged_plan(const vlt5_paged_attn_desc* d, const PagedSeqs& s) {
     const int g = d->H / d->kv.n_kv_heads;
     const long long rows = (long long)s.max_q * g;
@@ -537,8 +624,11 @@ PagedPlan paged_plan(const vlt5_paged_attn_desc* d, const PagedSeqs& s) {
     p.row_tiles = (int)((rows + per - 1) / per);
     const long long most_kv = d->max_kv > 0 ? d->max_kv : (long long)d->seqs.max_pages * d->kv.page_size;
     const long long tiles = (long long)s.B * d->kv.n_kv_heads * p.row_tiles;
-    long long sp = ((p.chunk ? 512 : 1024) + tiles - 1) / tiles;
-    sp = sp < most_kv / 512 ? sp : most_kv / 512;
+    static const int TG = getenv("PAT") ? atoi(getenv("PAT")) : 1024, MN = getenv("PAM") ? atoi(getenv("PAM")) : 512;
+    long long sp = ((p.chunk ? 512 : TG) + tiles - 1) / tiles;
+    sp = sp < most_kv / MN ? sp : most_kv / MN;
+    static const int W = getenv("PAW") ? atoi(getenv("PAW")) : 0;
+    p.waves = W ? W : (most_kv <= 128 ? 1 : 4);
     p.splits = (int)(sp < 1 ? 1 : (sp > 64 ? 64 : sp));
     return p;
 }
@@ -572,7 +662,7 @@ extern "C" int vlt5_paged_attn(const vlt5_paged_attn_desc* d, void* stream) {
     a.H = d->H; a.Hkv = c.n_kv_heads; a.g = d->H / c.n_kv_heads;
     a.scale = d->scale; a.causal = d->causal; a.bias = d->rel_bias; a.nd = d->n_dist;
     const PagedPlan plan = paged_plan(d, a.s);
-    a.row_tiles = plan.row_tiles; a.splits = plan.splits; a.join_tiles = (int)(((long long)a.s.max_q * a.g + 15) / 16);
+    a.row_tiles = plan.row_tiles; a.splits = plan.splits;
     const long long rows = (long long)a.s.n_tok * a.H;
     if (a.splits > 1) {
         if (!d->workspace || d->workspace_bytes < (long long)a.splits * rows * (c.d_kv + 2) * 4) return VLT5_ERR_ARG;
@@ -582,11 +672,13 @@ extern "C" int vlt5_paged_attn(const vlt5_paged_attn_desc* d, void* stream) {
         a.part_o = a.part_ml = nullptr;
     }
     const long long tiles = (long long)a.s.B * a.Hkv * a.row_tiles;
-    const long long joins = (long long)a.s.B * a.Hkv * a.join_tiles;
+    const int wpr = a.splits > 8 ? 4 : 1;                                           // waves that join a row
+    const long long joins = ((long long)a.s.B * a.H * a.s.max_q * wpr + 3) / 4;
     if (tiles * a.splits > 0x7fffffffLL || joins > 0x7fffffffLL) return VLT5_ERR_ARG;
     hipStream_t st = (hipStream_t)stream;
     int lrc = VLT5_OK;
 #define PA(T, D) do { if (plan.chunk) lrc = a.bias ? chunk_launch<T, D, true>(a, (unsigned)(tiles * a.splits), st) : chunk_launch<T, D, false>(a, (unsigned)(tiles * a.splits), st); \
+                      else if (plan.waves == 1) hipLaunchKernelGGL((paged_attn_kernel<T, D, 1>), dim3((unsigned)(tiles * a.splits)), dim3(64), 0, st, a); \
                       else hipLaunchKernelGGL((paged_attn_kernel<T, D, 4>), dim3((unsigned)(tiles * a.splits)), dim3(256), 0, st, a); } while (0)
     if (c.d_kv == 64) {
         if (c.type == VLT5_KV_BF16) PA(VLT5_KV_BF16, 64); else if (c.type == VLT5_KV_INT8) PA(VLT5_KV_INT8, 64); else PA(VLT5_KV_FP8, 64);
@@ -597,8 +689,10 @@ extern "C" int vlt5_paged_attn(const vlt5_paged_attn_desc* d, void* stream) {
     if (lrc) return lrc;
     LAUNCH_CHECK();
     if (a.splits > 1) {
-        if (c.d_kv == 64) hipLaunchKernelGGL(paged_join_kernel<64>, dim3((unsigned)joins), dim3(256), 0, st, a);
-        else hipLaunchKernelGGL(paged_join_kernel<128>, dim3((unsigned)joins), dim3(256), 0, st, a);
+#define PJ(D, W) hipLaunchKernelGGL((paged_join_kernel<D, W>), dim3((unsigned)joins), dim3(256), 0, st, a)
+        if (c.d_kv == 64) { if (wpr == 4) PJ(64, 4); else PJ(64, 1); }
+        else { if (wpr == 4) PJ(128, 4); else PJ(128, 1); }
+#undef PJ
         LAUNCH_CHECK();
     }
     return VLT5_OK;
