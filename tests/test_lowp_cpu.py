@@ -92,7 +92,7 @@ def test_attention_refusals(built):
         assert L.vlt5_paged_attn_workspace_bytes(C.byref(desc(kv=change))) == -1
     for change, rc in BAD_SEQ:
         assert L.vlt5_paged_attn(C.byref(desc(seq=change)), None) == rc, change
-    for change, rc in (({"q": None}, ARG), ({"out": None}, ARG), ({"H": 3}, ARG), ({"H": 0}, ARG), ({"q_st": 255}, ARG), ({"o_st": 128}, ARG), ({"rel_bias": P}, ARG),
+    for change, rc in (({"q": None}, ARG), ({"out": None}, ARG), ({"H": 3}, ARG), ({"H": 0}, ARG), ({"q_st": 255}, ARG), ({"o_st": 128}, ARG), ({"rel_bias": P}, ARG), ({"scale": 0.0}, ARG), ({"scale": -1.0}, ARG), ({"scale": float("nan")}, ARG), ({"scale": float("inf")}, ARG),
                        ({"rel_bias": P, "n_dist": 4, "causal": 0}, ARG), ({"q_st": 260}, ALIGN), ({"q": P + 2}, ALIGN), ({"out": P + 8}, ALIGN), ({"workspace": P + 4}, ALIGN)):
         assert L.vlt5_paged_attn(C.byref(desc(**change)), None) == rc, change
     # a long context of few sequences is shared out and needs a workspace of its own: too small is refused

@@ -28,6 +28,14 @@ struct PagedAttnArgs {
     float* part_o; float* part_ml;            // [splits][n_tok * H][d_kv], [splits][n_tok * H][2]
 };
 
+// Makes the compiler wait for a loaded operand HERE: left to its first use inside a loop, the wait would be repeated in every pass and hold up
+// the loads of the pass after (they are counted in order).
+template <class V>
+__device__ __forceinline__ void arrived(V& f) { asm volatile("" : "+v"(f)); }
+
+// The bias of a row tile's heads is read from LDS where it fits this many entries: a gather from memory would wait for the keys requested before it.
+constexpr int BIAS_LDS = 1024;
+
 constexpr float LOG2E = 1.4426950408889634f;
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -108,10 +116,18 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_kernel(const PagedAttnA
     const bf16_t* qrow = a.q + (size_t)(sq.q0 + tok) * a.q_st + hq * DK;
 #pragma unroll
     for (int i = 0; i < NF; ++i) fq[i] = *reinterpret_cast<const bf16x8_t*>(qrow + (T == VLT5_KV_BF16 ? i * 32 + kq * 8 : (i >> 1) * 64 + kq * 16 + (i & 1) * 8));
+    __shared__ float sb[BIAS_LDS];
+    const bool near_lds = a.bias && a.g * a.nd <= BIAS_LDS;
+    if (near_lds) {
+        for (int i = threadIdx.x; i < a.g * a.nd; i += NW * 64) sb[i] = a.bias[(size_t)hk * a.g * a.nd + i];
+        __syncthreads();
+    }
     const float* bias = a.bias ? a.bias + (size_t)hq * a.nd : nullptr;
-    const float bias_far = bias ? bias[a.nd - 1] : 0.f;
-    const float unit = bias ? 1.f : LOG2E, rest = bias ? LOG2E : 1.f;              // without a bias scores are kept in powers of two
-    const float cs = a.scale * unit;
+    const float* lbias = sb + (hq - hk * a.g) * a.nd;
+    float bias_far = bias ? bias[a.nd - 1] : 0.f;
+    arrived(bias_far);
+    // scores and their maximum are kept as q k (times the key's scale), with a bias as scale * q k + bias; `unit` makes powers of two of them
+    const float unit = bias ? LOG2E : a.scale * LOG2E, lag = 8.f / unit;
 
     f32x4_t o[ND];
 #pragma unroll
@@ -123,6 +139,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_kernel(const PagedAttnA
     auto load_ids = [&](int i) {
         const int t = at(i + (lane >> 1)) + (lane & 1) * 16;
         ids = i + (lane >> 1) < mine && t < hi ? paged_page(a.s, b, t) : -1;
+        arrived(ids);
     };
     int pg[2][2];
     KeyStep<T, DK> st[2];
@@ -156,22 +173,28 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_kernel(const PagedAttnA
             float kk[4] = {1.f, 1.f, 1.f, 1.f};
             if constexpr (KvType<T>::SCALED) { kk[0] = x.ks[i].x; kk[1] = x.ks[i].y; kk[2] = x.ks[i].z; kk[3] = x.ks[i].w; }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) p[i][e] = sc[i][e] * (kk[e] * cs);
+            for (int e = 0; e < 4; ++e) p[i][e] = sc[i][e] * kk[e];
         }
         if (bias) {
             if (first - (t0 + 31) >= a.nd - 1) {                                   // every key further than the table reaches
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) p[i][e] += bias_far;
+                    for (int e = 0; e < 4; ++e) p[i][e] = fmaf(p[i][e], a.scale, bias_far);
+            } else if (near_lds) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[i][e] = fmaf(p[i][e], a.scale, lbias[min(max(pos - (t0 + i * 16 + kq * 4 + e), 0), a.nd - 1)]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) p[i][e] += bias[min(max(pos - (t0 + i * 16 + kq * 4 + e), 0), a.nd - 1)];
+                    for (int e = 0; e < 4; ++e) p[i][e] = fmaf(p[i][e], a.scale, bias[min(max(pos - (t0 + i * 16 + kq * 4 + e), 0), a.nd - 1)]);
             }
         }
         if (!whole) {
+            asm volatile("");                                                      // (a branch, not selects in every step)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -183,11 +206,11 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_kernel(const PagedAttnA
             for (int e = 0; e < 4; ++e) top = fmaxf(top, p[i][e]);
         // the running maximum moves only when a new one is more than 2^8 away: until then probabilities up to 256 do no harm (f32 sums, bf16
         // relative to the value), and neither the exchange between the row's four lanes nor the rescaling is needed
-        if (__any(top > m + 8.f * (unit / LOG2E))) {
+        if (__any(top > m + lag)) {
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64));
             const float mn = fmaxf(m, top), ms = mn == -INFINITY ? 0.f : mn;        // a row that has seen no key yet stays at -inf, sum 0
-            const float fix = exp2_hw((m - ms) * rest);
+            const float fix = exp2_hw((m - ms) * unit);
             m = mn;
             l *= fix;
 #pragma unroll
@@ -203,7 +226,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_kernel(const PagedAttnA
             if constexpr (KvType<T>::SCALED) { vv[0] = x.vs[i].x; vv[1] = x.vs[i].y; vv[2] = x.vs[i].z; vv[3] = x.vs[i].w; }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float pe = exp2_hw((p[i][e] - ms) * rest);
+                const float pe = exp2_hw((p[i][e] - ms) * unit);
                 l += pe;
                 y[e] = pe * vv[e];
             }
@@ -231,18 +254,26 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_kernel(const PagedAttnA
         load_ids(0);
         load(0, 0);
     }
-    for (int i = 0; i < mine; i += 2) {
-        if (i + 1 < mine) load(i + 1, 1);                                          // (i is even: never the first of 32 steps)
+#pragma unroll
+    for (int i = 0; i < NF; ++i) arrived(fq[i]);
+    int i = 0;
+    for (; i + 2 < mine; i += 2) {                                                 // (every load unconditional, or the waits could not be counted)
+        load(i + 1, 1);                                                            // (i is even: never the first of 32 steps)
         use(i, 0);
-        if (i + 2 < mine) {
-            if (((i + 2) & 31) == 0) load_ids(i + 2);
-            load(i + 2, 0);
-        }
-        if (i + 1 < mine) use(i + 1, 1);
+        if (((i + 2) & 31) == 0) load_ids(i + 2);
+        load(i + 2, 0);
+        use(i + 1, 1);
+    }
+    if (i + 1 < mine) {
+        load(i + 1, 1);
+        use(i, 0);
+        use(i + 1, 1);
+    } else if (i < mine) {
+        use(i, 0);
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-    m = bias ? m : m / LOG2E;
+    m = bias ? m : m * a.scale;
 
     // ---- the waves' shares of the keys meet in LDS, always in the order of the waves ----
     __shared__ float so[NW][16][DK + 4];
@@ -325,9 +356,15 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
 #pragma unroll
     for (int i = 0; i < NKS; ++i) fq[i] = *reinterpret_cast<const bf16x8_t*>(qrow + i * 16 + h * 8);
     const float* bias = BIAS ? a.bias + (size_t)hq * a.nd : nullptr;
-    const float bias_far = BIAS ? bias[a.nd - 1] : 0.f;
-    const float unit = BIAS ? 1.f : LOG2E;                                              // without a bias scores are kept in powers of two
-    const float cs = a.scale * unit;
+    float bias_far = BIAS ? bias[a.nd - 1] : 0.f;
+    arrived(bias_far);
+    float* sb = reinterpret_cast<float*>(smem + 2 * BUF);
+    const bool near_lds = BIAS && a.g * a.nd <= BIAS_LDS;
+    const float* lbias = sb + (hq - hk * a.g) * a.nd;
+    if (near_lds)
+        for (int i = tid; i < a.g * a.nd; i += 256) sb[i] = a.bias[(size_t)hk * a.g * a.nd + i];      // (the barrier before the first tile covers it)
+    // scores and their maximum are kept as q k (times the key's scale), with a bias as scale * q k + bias; `unit` makes powers of two of them
+    const float unit = BIAS ? LOG2E : a.scale * LOG2E, lag = 8.f / unit;
 
     // ---- one tile's raw rows on their way ----
     vlt5_u32x4_t kr[KP];
@@ -339,6 +376,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
     auto load_ids = [&](int tile) {
         const int t = lo + tile * 64 + lane * 16;
         ids = t < hi ? paged_page(a.s, b, t) : -1;
+        arrived(ids);
     };
     auto first_row = [&](int page, int t) { return (((size_t)max(page, 0) * a.Hkv + hk) << a.s.page_shift) + (t & ((1 << a.s.page_shift) - 1)); };
     auto fetch = [&](int tile) {
@@ -417,6 +455,8 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
         fetch(0);
         stage(smem);
     }
+#pragma unroll
+    for (int i = 0; i < NKS; ++i) arrived(fq[i]);
     __syncthreads();
     for (int tile = 0; tile < tiles; ++tile) {
         const int t0 = lo + tile * 64, cur = tile & 1;
@@ -440,53 +480,53 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
             }
             // register e of tile i: key t0 + i * 32 + 8 * (e / 4) + 4 * h + e % 4
             const bool whole = t0 + 64 <= wLmin && min(min(pg[0], pg[1]), min(pg[2], pg[3])) >= 0;
-            const bool far = BIAS && p0 + min(wr0, rows - 1) / a.g - (t0 + 63) >= a.nd - 1;      // every key further than the table reaches
             const float* ks = reinterpret_cast<const float*>(buf + KBYTES + VBYTES);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    float4 k4 = make_float4(1.f, 1.f, 1.f, 1.f);
-                    if constexpr (KvType<T>::SCALED) k4 = *reinterpret_cast<const float4*>(ks + i * 32 + q * 8 + h * 4);
-                    const float kk[4] = {k4.x, k4.y, k4.z, k4.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[i][q * 4 + e] *= KvType<T>::SCALED ? kk[e] * cs : cs;
-                    }
-                }
-            if constexpr (BIAS) {
-                if (far) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) s[i][e] += bias_far;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) s[i][e] += bias[min(max(pos - (t0 + i * 32 + e / 4 * 8 + h * 4 + e % 4), 0), a.nd - 1)];
-                }
-            }
-            if (!whole) {
+            if constexpr (KvType<T>::SCALED) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        const bool page = pg[i * 2 + q / 2] >= 0;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            s[i][q * 4 + e] = page && t0 + i * 32 + q * 8 + h * 4 + e < L ? s[i][q * 4 + e] : -INFINITY;
+                        const float4 k4 = *reinterpret_cast<const float4*>(ks + i * 32 + q * 8 + h * 4);
+                        s[i][q * 4] *= k4.x; s[i][q * 4 + 1] *= k4.y; s[i][q * 4 + 2] *= k4.z; s[i][q * 4 + 3] *= k4.w;
                     }
+            }
+            if constexpr (BIAS) {
+                if (p0 + min(wr0, rows - 1) / a.g - (t0 + 63) >= a.nd - 1) {            // every key further than the table reaches
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s[i][e] = fmaf(s[i][e], a.scale, bias_far);
+                } else if (near_lds) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            s[i][e] = fmaf(s[i][e], a.scale, lbias[min(max(pos - (t0 + i * 32 + e / 4 * 8 + h * 4 + e % 4), 0), a.nd - 1)]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            s[i][e] = fmaf(s[i][e], a.scale, bias[min(max(pos - (t0 + i * 32 + e / 4 * 8 + h * 4 + e % 4), 0), a.nd - 1)]);
+                }
+            }
+            if (!whole) {
+                asm volatile("");                                                       // (a branch, not 96 instructions of selects in every tile)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        s[i][e] = pg[i * 2 + e / 8] >= 0 && t0 + i * 32 + e / 4 * 8 + h * 4 + e % 4 < L ? s[i][e] : -INFINITY;
             }
             float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) top = fmaxf(top, s[i][e]);
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            if (__any(top > m + 8.f * unit / LOG2E)) {
+            if (__any(top > m + lag)) {
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
                 const float mn = fmaxf(m, top), ms = mn == -INFINITY ? 0.f : mn;
-                const float fix = exp2_hw((m - ms) * (BIAS ? LOG2E : 1.f));
+                const float fix = exp2_hw((m - ms) * unit);
                 m = mn;
                 l *= fix;
 #pragma unroll
@@ -494,7 +534,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
 #pragma unroll
                     for (int e = 0; e < 16; ++e) o[j][e] *= fix;
             }
-            const float ms = m == -INFINITY ? 0.f : m;
+            const float ms = m == -INFINITY ? 0.f : m, mu = -ms * unit;
             bf16x8_t fp[4];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -503,16 +543,17 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
                     uint32_t pk[4];
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
-                        float4 v4 = make_float4(1.f, 1.f, 1.f, 1.f);
-                        if constexpr (KvType<T>::SCALED) v4 = *reinterpret_cast<const float4*>(ks + 64 + i * 32 + (g2 * 2 + q) * 8 + h * 4);
-                        const float vv[4] = {v4.x, v4.y, v4.z, v4.w};
                         float x[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const float d = s[i][(g2 * 2 + q) * 4 + e] - ms;
-                            const float pe = exp2_hw(BIAS ? d * LOG2E : d);
-                            l += pe;
-                            x[e] = KvType<T>::SCALED ? pe * vv[e] : pe;
+                            const float z = s[i][(g2 * 2 + q) * 4 + e];
+                            // (with a bias not one fused operation: the type's lowest value as a mask times log2(e) would leave the range)
+                            x[e] = exp2_hw(BIAS ? (z - ms) * LOG2E : fmaf(z, unit, mu));
+                            l += x[e];
+                        }
+                        if constexpr (KvType<T>::SCALED) {
+                            const float4 v4 = *reinterpret_cast<const float4*>(ks + 64 + i * 32 + (g2 * 2 + q) * 8 + h * 4);
+                            x[0] *= v4.x; x[1] *= v4.y; x[2] *= v4.z; x[3] *= v4.w;
                         }
                         pk[q * 2] = pack_bf16x2(x[0], x[1]);
                         pk[q * 2 + 1] = pack_bf16x2(x[2], x[3]);
@@ -531,7 +572,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
     }
     l += __shfl_xor(l, 32, 64);
     if (wr0 + r32 >= rows) return;
-    const float mnat = BIAS ? m : m / LOG2E;
+    const float mnat = BIAS ? m : m * a.scale;
     const size_t row = (size_t)(sq.q0 + tok) * a.H + hq;
     if (a.splits == 1) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -608,7 +649,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
 template <int T, int DK, bool BIAS>
 int chunk_launch(const PagedAttnArgs& a, unsigned blocks, hipStream_t st) {
     static std::atomic<unsigned long long> done{0};
-    constexpr int bytes = 2 * (64 * (DK * 2 + 16) + 4 * (DK / 32) * 1024 + 512);
+    constexpr int bytes = 2 * (64 * (DK * 2 + 16) + 4 * (DK / 32) * 1024 + 512) + (BIAS ? BIAS_LDS * 4 : 0);
     const int rc = vlt5_lds_optin((const void*)paged_chunk_kernel<T, DK, BIAS>, bytes, done);
     if (rc) return rc;
     hipLaunchKernelGGL((paged_chunk_kernel<T, DK, BIAS>), dim3(blocks), dim3(256), bytes, st, a);
@@ -653,6 +694,7 @@ extern "C" int vlt5_paged_attn(const vlt5_paged_attn_desc* d, void* stream) {
     if (d->H <= 0 || d->H % c.n_kv_heads || d->H > 1024) return VLT5_ERR_ARG;
     if (d->q_st < (long long)d->H * c.d_kv || d->o_st < (long long)d->H * c.d_kv) return VLT5_ERR_ARG;
     if (d->rel_bias && (d->n_dist <= 0 || !d->causal)) return VLT5_ERR_ARG;
+    if (!(d->scale > 0.f && d->scale <= 3.402823466e38f)) return VLT5_ERR_ARG;
     if ((d->q_st & 7) || (d->o_st & 7) || (((uintptr_t)d->q | (uintptr_t)d->out | (uintptr_t)d->workspace) & 15)) return VLT5_ERR_ALIGN;
     if (d->seqs.n_tok == 0) return VLT5_OK;
     PagedAttnArgs a;
