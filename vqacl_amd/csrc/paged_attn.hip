@@ -10,7 +10,6 @@
 // 8-bit codes are exact in bf16; the scale of a key multiplies its score, the scale of a value its probability (in f32, before the one
 // rounding of the probabilities to bf16).
 #include "paged.h"
-#include <stdlib.h>
 
 namespace {
 
@@ -324,14 +323,15 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_kernel(const PagedAttnA
 // type they pass through (f32 sums, bf16 relative to the value), and the output's 16 * NT registers are left alone.
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 
-template <int T, int DK, bool BIAS>
-__global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs a) {
+template <int T, int DK, bool BIAS, int KS>
+__global__ __launch_bounds__(256 * KS, 2) void paged_chunk_kernel(const PagedAttnArgs a) {
     constexpr int NT = DK / 32, NKS = DK / 16, BY = KvType<T>::BYTES, ROWB = DK * BY;
     constexpr int KROW = DK * 2 + 16, KBYTES = 64 * KROW, VBYTES = 4 * NT * 1024, BUF = KBYTES + VBYTES + 512;
     constexpr int KCH = ROWB / 16, KP = 64 * KCH / 256;                                 // 16-byte pieces of a key row; pieces of a thread
     constexpr int VW = (NT * BY + 3) / 4;                                               // dwords of a thread's share of a value row
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r32 = lane & 31, h = lane >> 5;
+    const int w4 = w & 3, half = w >> 2;                                                // wave of its half, half
     const int pairs = a.s.B * a.Hkv;
     const int pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
     const int sp = rest % a.splits, rt = a.row_tiles - 1 - rest / a.splits;             // the last rows see the most keys: they start first
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
     const PagedSeq sq = paged_seq(a.s, b);
     const int rows = min(sq.nq, a.s.max_q) * a.g;
     if (rt * 128 >= rows) return;
-    const int wr0 = rt * 128 + w * 32;                                                  // first row of the wave
+    const int wr0 = rt * 128 + w4 * 32;                                                 // first row of the wave
     const int r = min(wr0 + r32, rows - 1);
     const int tok = r / a.g, hq = hk * a.g + r % a.g;
     const int pos = sq.len - sq.nq + tok;
@@ -358,11 +358,11 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
     const float* bias = BIAS ? a.bias + (size_t)hq * a.nd : nullptr;
     float bias_far = BIAS ? bias[a.nd - 1] : 0.f;
     arrived(bias_far);
-    float* sb = reinterpret_cast<float*>(smem + 2 * BUF);
+    float* sb = reinterpret_cast<float*>(smem + 2 * KS * BUF);
     const bool near_lds = BIAS && a.g * a.nd <= BIAS_LDS;
     const float* lbias = sb + (hq - hk * a.g) * a.nd;
     if (near_lds)
-        for (int i = tid; i < a.g * a.nd; i += 256) sb[i] = a.bias[(size_t)hk * a.g * a.nd + i];      // (the barrier before the first tile covers it)
+        for (int i = tid; i < a.g * a.nd; i += 256 * KS) sb[i] = a.bias[(size_t)hk * a.g * a.nd + i];      // (the barrier before the first tile covers it)
     // scores and their maximum are kept as q k (times the key's scale), with a bias as scale * q k + bias; `unit` makes powers of two of them
     const float unit = BIAS ? LOG2E : a.scale * LOG2E, lag = 8.f / unit;
 
@@ -386,12 +386,12 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
             // the pieces of 64 lanes are 64 / KCH (4, 8 or 16) keys of one group of 16
-            const int base = (i * 256 + w * 64) / KCH, grp = base >> 4;
+            const int base = (i * 256 + w4 * 64) / KCH, grp = base >> 4;
             const int page = grp == 0 ? pn[0] : (grp == 1 ? pn[1] : (grp == 2 ? pn[2] : pn[3]));
             kr[i] = *reinterpret_cast<const vlt5_u32x4_t*>(a.k + (first_row(page, t0 + grp * 16) + ((base & 15) + lane / KCH)) * ROWB + (lane % KCH) * 16);
         }
-        const int g0 = w == 0 ? pn[0] : (w == 1 ? pn[1] : (w == 2 ? pn[2] : pn[3]));
-        const unsigned char* vp = a.v + first_row(g0, t0 + w * 16) * ROWB + r32 * (NT * BY);
+        const int g0 = w4 == 0 ? pn[0] : (w4 == 1 ? pn[1] : (w4 == 2 ? pn[2] : pn[3]));
+        const unsigned char* vp = a.v + first_row(g0, t0 + w4 * 16) * ROWB + r32 * (NT * BY);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const unsigned char* p = vp + (size_t)((e >> 2) * 8 + h * 4 + (e & 3)) * ROWB;
@@ -400,17 +400,18 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
             else vr[e][0] = *reinterpret_cast<const uint16_t*>(p);
         }
         if constexpr (KvType<T>::SCALED) {
-            if (w < 2) {                                                                // wave 0: key scales, wave 1: value scales
+            const bool ws = w4 == 1;                                                    // wave 0: key scales, wave 1: value scales
+            if (w4 < 2) {
                 const int page = lane < 16 ? pn[0] : (lane < 32 ? pn[1] : (lane < 48 ? pn[2] : pn[3]));
-                scl = (w ? a.vs : a.ks)[first_row(page, t0 + lane)];
-                if (w && (page < 0 || t0 + lane >= sq.len)) scl = 0.f;
+                scl = (ws ? a.vs : a.ks)[first_row(page, t0 + lane)];
+                if (ws && (page < 0 || t0 + lane >= sq.len)) scl = 0.f;
             }
         }
         // what lies behind the last key or in a page that is not there may hold anything, NaN too
-        if (t0 + w * 16 + 16 > sq.len || g0 < 0) {
+        if (t0 + w4 * 16 + 16 > sq.len || g0 < 0) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (g0 < 0 || t0 + w * 16 + (e >> 2) * 8 + h * 4 + (e & 3) >= sq.len)
+                if (g0 < 0 || t0 + w4 * 16 + (e >> 2) * 8 + h * 4 + (e & 3) >= sq.len)
 #pragma unroll
                     for (int i = 0; i < VW; ++i) vr[e][i] = 0;
         }
@@ -418,7 +419,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
     auto stage = [&](char* buf) {
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
-            char* p = buf + ((i * 256 + w * 64) / KCH + lane / KCH) * KROW + (lane % KCH) * (16 / BY * 2);
+            char* p = buf + ((i * 256 + w4 * 64) / KCH + lane / KCH) * KROW + (lane % KCH) * (16 / BY * 2);
             if constexpr (T == VLT5_KV_BF16) {
                 *reinterpret_cast<vlt5_u32x4_t*>(p) = kr[i];
             } else {
@@ -438,10 +439,10 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
                 else if constexpr (T == VLT5_KV_INT8) q[e] = pack_bf16x2(sbyte(x, j), sbyte(y, j));
                 else q[e] = cvt_fp8_pair(__builtin_amdgcn_perm(y, x, j & 2 ? 0x07030602u : 0x05010400u), j & 1);
             }
-            *reinterpret_cast<uint4*>(v + ((w * NT + j) * 64 + lane) * 16) = make_uint4(q[0], q[1], q[2], q[3]);
+            *reinterpret_cast<uint4*>(v + ((w4 * NT + j) * 64 + lane) * 16) = make_uint4(q[0], q[1], q[2], q[3]);
         }
         if constexpr (KvType<T>::SCALED)
-            if (w < 2) reinterpret_cast<float*>(v + VBYTES)[w * 64 + lane] = scl;
+            if (w4 < 2) reinterpret_cast<float*>(v + VBYTES)[w4 * 64 + lane] = scl;
     };
 
     f32x16_t o[NT];
@@ -450,25 +451,26 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[j][e] = 0.f;
     float m = -INFINITY, l = 0.f;
-    if (tiles > 0) {
+    char* mine = smem + half * 2 * BUF;
+    if (half < tiles) {
         load_ids(0);
-        fetch(0);
-        stage(smem);
+        fetch(half);
+        stage(mine);
     }
 #pragma unroll
     for (int i = 0; i < NKS; ++i) arrived(fq[i]);
     __syncthreads();
-    for (int tile = 0; tile < tiles; ++tile) {
-        const int t0 = lo + tile * 64, cur = tile & 1;
-        const char* buf = smem + cur * BUF;
-        const bool more = tile + 1 < tiles;
+    for (int turn = 0; turn * KS < tiles; ++turn) {
+        const int tile = turn * KS + half, t0 = lo + tile * 64, cur = turn & 1;
+        const char* buf = mine + cur * BUF;
+        const bool more = tile + KS < tiles;
 #pragma unroll
         for (int i = 0; i < 4; ++i) pg[i] = pn[i];
         if (more) {
-            if (((tile + 1) & 15) == 0) load_ids(tile + 1);
-            fetch(tile + 1);
+            if (((tile + KS) & 15) == half) load_ids((tile + KS) & ~15);
+            fetch(tile + KS);
         }
-        if (t0 < wLmax) {
+        if (t0 < wLmax && tile < tiles) {
             f32x16_t s[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -500,14 +502,18 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e)
+                        for (int e = 0; e < 16; ++e) {
                             s[i][e] = fmaf(s[i][e], a.scale, lbias[min(max(pos - (t0 + i * 32 + e / 4 * 8 + h * 4 + e % 4), 0), a.nd - 1)]);
+                            if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);          // (all 32 in flight would not leave registers for the sums)
+                        }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e)
+                        for (int e = 0; e < 16; ++e) {
                             s[i][e] = fmaf(s[i][e], a.scale, bias[min(max(pos - (t0 + i * 32 + e / 4 * 8 + h * 4 + e % 4), 0), a.nd - 1)]);
+                            if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                        }
                 }
             }
             if (!whole) {
@@ -567,10 +573,32 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnArgs
                 for (int j = 0; j < NT; ++j)
                     o[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(v + ((g2 * NT + j) * 64 + lane) * 16), fp[g2], o[j], 0, 0, 0);
         }
-        if (more) stage(smem + (cur ^ 1) * BUF);
+        if (more) stage(mine + (cur ^ 1) * BUF);
         __syncthreads();
     }
     l += __shfl_xor(l, 32, 64);
+    if constexpr (KS == 2) {
+        // the second half's sums go to the first through LDS (nobody reads tiles any more), register by register
+        float* x = reinterpret_cast<float*>(smem) + w4 * (16 * NT + 2) * 64 + lane;
+        if (half) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[(j * 16 + e) * 64] = o[j][e];
+            x[16 * NT * 64] = m;
+            x[(16 * NT + 1) * 64] = l;
+        }
+        __syncthreads();
+        if (half) return;
+        const float m1 = x[16 * NT * 64], mn = fmaxf(m, m1), ms = mn == -INFINITY ? 0.f : mn;
+        const float f0 = exp2_hw((m - ms) * unit), f1 = exp2_hw((m1 - ms) * unit);
+        m = mn;
+        l = l * f0 + x[(16 * NT + 1) * 64] * f1;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[j][e] = o[j][e] * f0 + x[(j * 16 + e) * 64] * f1;
+    }
     if (wr0 + r32 >= rows) return;
     const float mnat = BIAS ? m : m * a.scale;
     const size_t row = (size_t)(sq.q0 + tok) * a.H + hq;
@@ -646,31 +674,35 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
     if (a.lse && lane == 0) a.lse[row] = sum == 0.f ? -INFINITY : mx + logf(sum);
 }
 
-template <int T, int DK, bool BIAS>
+template <int T, int DK, bool BIAS, int KS>
 int chunk_launch(const PagedAttnArgs& a, unsigned blocks, hipStream_t st) {
     static std::atomic<unsigned long long> done{0};
-    constexpr int bytes = 2 * (64 * (DK * 2 + 16) + 4 * (DK / 32) * 1024 + 512) + (BIAS ? BIAS_LDS * 4 : 0);
-    const int rc = vlt5_lds_optin((const void*)paged_chunk_kernel<T, DK, BIAS>, bytes, done);
+    constexpr int bytes = 2 * KS * (64 * (DK * 2 + 16) + 4 * (DK / 32) * 1024 + 512) + (BIAS ? BIAS_LDS * 4 : 0);
+    const int rc = vlt5_lds_optin((const void*)paged_chunk_kernel<T, DK, BIAS, KS>, bytes, done);
     if (rc) return rc;
-    hipLaunchKernelGGL((paged_chunk_kernel<T, DK, BIAS>), dim3(blocks), dim3(256), bytes, st, a);
+    hipLaunchKernelGGL((paged_chunk_kernel<T, DK, BIAS, KS>), dim3(blocks), dim3(256 * KS), bytes, st, a);
     return VLT5_OK;
 }
+
+// The plan of a call, from what the host knows.  Up to 64 rows (tokens x heads of a group) go through the first kernel, more share their keys
+// through LDS.  A row tile's keys are shared by one wave up to 128 of them, else by four (80 sequences x 58 keys, 12 heads: 6.0 against 8.0 us;
+// 100 x 500: 20.4 against 19.1), and by as many workgroups as give every CU two, none with less than 512 keys (1 x 131071 keys, 8 kv heads of 128,
+// int8: 67 us in 64 shares; 8 x 2000 keys: 15 us in 3 shares of 667, 17 in 7 of 286).  Large tiles that leave a CU one workgroup get twice the
+// waves, half the keys each (8 sequences of 200 tokens over 712 keys, 12 heads: 28.4 -> 20.5 us; where CUs have two anyway it costs 5 %).
 struct PagedPlan { int chunk, row_tiles, splits, waves; };
 PagedPlan paged_plan(const vlt5_paged_attn_desc* d, const PagedSeqs& s) {
     const int g = d->H / d->kv.n_kv_heads;
     const long long rows = (long long)s.max_q * g;
+    const long long most_kv = d->max_kv > 0 ? d->max_kv : (long long)d->seqs.max_pages * d->kv.page_size;
     PagedPlan p;
     p.chunk = rows > 64;
     const int per = p.chunk ? 128 : 16;
     p.row_tiles = (int)((rows + per - 1) / per);
-    const long long most_kv = d->max_kv > 0 ? d->max_kv : (long long)d->seqs.max_pages * d->kv.page_size;
     const long long tiles = (long long)s.B * d->kv.n_kv_heads * p.row_tiles;
-    static const int TG = getenv("PAT") ? atoi(getenv("PAT")) : 1024, MN = getenv("PAM") ? atoi(getenv("PAM")) : 512;
-    long long sp = ((p.chunk ? 512 : TG) + tiles - 1) / tiles;
-    sp = sp < most_kv / MN ? sp : most_kv / MN;
-    static const int W = getenv("PAW") ? atoi(getenv("PAW")) : 0;
-    p.waves = W ? W : (most_kv <= 128 ? 1 : 4);
+    long long sp = (512 + tiles - 1) / tiles;
+    sp = sp < most_kv / 512 ? sp : most_kv / 512;
     p.splits = (int)(sp < 1 ? 1 : (sp > 64 ? 64 : sp));
+    p.waves = p.chunk ? (tiles * p.splits <= 256 ? 8 : 4) : (most_kv <= 128 ? 1 : 4);
     return p;
 }
 
@@ -719,7 +751,8 @@ extern "C" int vlt5_paged_attn(const vlt5_paged_attn_desc* d, void* stream) {
     if (tiles * a.splits > 0x7fffffffLL || joins > 0x7fffffffLL) return VLT5_ERR_ARG;
     hipStream_t st = (hipStream_t)stream;
     int lrc = VLT5_OK;
-#define PA(T, D) do { if (plan.chunk) lrc = a.bias ? chunk_launch<T, D, true>(a, (unsigned)(tiles * a.splits), st) : chunk_launch<T, D, false>(a, (unsigned)(tiles * a.splits), st); \
+#define PA(T, D) do { if (plan.chunk && plan.waves == 8) lrc = a.bias ? chunk_launch<T, D, true, 2>(a, (unsigned)(tiles * a.splits), st) : chunk_launch<T, D, false, 2>(a, (unsigned)(tiles * a.splits), st); \
+                      else if (plan.chunk) lrc = a.bias ? chunk_launch<T, D, true, 1>(a, (unsigned)(tiles * a.splits), st) : chunk_launch<T, D, false, 1>(a, (unsigned)(tiles * a.splits), st); \
                       else if (plan.waves == 1) hipLaunchKernelGGL((paged_attn_kernel<T, D, 1>), dim3((unsigned)(tiles * a.splits)), dim3(64), 0, st, a); \
                       else hipLaunchKernelGGL((paged_attn_kernel<T, D, 4>), dim3((unsigned)(tiles * a.splits)), dim3(256), 0, st, a); } while (0)
     if (c.d_kv == 64) {
