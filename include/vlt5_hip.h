@@ -731,8 +731,9 @@ int vlt5_kv_page_read(const vlt5_paged_kv* c, const vlt5_paged_seqs* q, int T, v
  * sees the positions up to its own, else all kv_lens[b].  rel_bias f32 [H][n_dist] (causal only): added to the score of a key that lies
  * `dist` positions back, the last entry for every larger dist -- T5's bucketed bias of a decoder as a function of the distance.  A token
  * that sees no key gets zeros and lse -inf.  lse (optional) f32 [n_tok][H].  max_kv: about the longest kv_lens (0 = the table's width); it
- * only decides how the work is split.  workspace: vlt5_paged_attn_workspace_bytes of the same desc (0: none needed), 16-byte aligned, one
- * per call in flight. */
+ * only decides how the work is split.  workspace: vlt5_paged_attn_workspace_bytes of the same desc (0: none needed, always so where max_kv or
+ * the table's width is below VLT5_PAGED_SHARED_KV), 16-byte aligned, one per call in flight. */
+#define VLT5_PAGED_SHARED_KV 1024
 typedef struct {
     vlt5_paged_kv kv; vlt5_paged_seqs seqs;
     const void* q; long long q_st; void* out; long long o_st; float* lse;

@@ -102,6 +102,10 @@ def test_attention_refusals(built):
     assert L.vlt5_paged_attn(C.byref(desc(**long)), None) == ARG
     assert L.vlt5_paged_attn(C.byref(desc(**long, workspace=P, workspace_bytes=need - 1)), None) == ARG
     assert L.vlt5_paged_attn_workspace_bytes(C.byref(desc())) == 0
+    edge = built.PAGED_SHARED_KV
+    assert f"#define VLT5_PAGED_SHARED_KV {edge}\n" in open(os.path.join(ROOT, "include", "vlt5_hip.h")).read()
+    assert L.vlt5_paged_attn_workspace_bytes(C.byref(desc(seq={"B": 1, "n_tok": 1, "max_pages": 4096}, max_kv=edge - 1))) == 0
+    assert L.vlt5_paged_attn_workspace_bytes(C.byref(desc(seq={"B": 1, "n_tok": 1, "max_pages": 4096}, max_kv=edge))) > 0
     assert L.vlt5_paged_attn(C.byref(desc(seq={"n_tok": 0})), None) == 0
 
 

@@ -305,6 +305,8 @@ PROTOTYPES = {
 
 WS_ENC_OUT, WS_ENC_EXT, WS_LOGITS, WS_LOSS_TOK, WS_LOSS, WS_ENC_MASK_EXT, WS_DEC_OUT = range(7)
 
+PAGED_SHARED_KV = 1024         # VLT5_PAGED_SHARED_KV
+
 _lib = None
 ABI_VERSION = 8
 BUILD_FLAG_NAMES = {1: "ENC_DGRAD_HOT_A (input-gradient GEMM reads one row: wrong gradients)", 2: "ATTN_BWD_NO_STORE (attention backward "

@@ -700,7 +700,7 @@ PagedPlan paged_plan(const vlt5_paged_attn_desc* d, const PagedSeqs& s) {
     p.row_tiles = (int)((rows + per - 1) / per);
     const long long tiles = (long long)s.B * d->kv.n_kv_heads * p.row_tiles;
     long long sp = (512 + tiles - 1) / tiles;
-    sp = sp < most_kv / 512 ? sp : most_kv / 512;
+    sp = sp < most_kv / (VLT5_PAGED_SHARED_KV / 2) ? sp : most_kv / (VLT5_PAGED_SHARED_KV / 2);
     p.splits = (int)(sp < 1 ? 1 : (sp > 64 ? 64 : sp));
     p.waves = p.chunk ? (tiles * p.splits <= 256 ? 8 : 4) : (most_kv <= 128 ? 1 : 4);
     return p;

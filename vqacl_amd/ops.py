@@ -359,7 +359,7 @@ def enc_attn_sublayer_bwd(dy, sv, want_dscores=False):
 
 
 # ---- the token-step in low precision: 4-bit weights, a paged key/value cache, the attention over it -------------------------------
-FP8 = torch.float8_e4m3fn
+FP8, F32, I32 = torch.float8_e4m3fn, torch.float32, torch.int32
 _KV_TYPE = {BF16: 0, torch.int8: 1, FP8: 2}
 
 
@@ -380,14 +380,14 @@ class KVPages(NamedTuple):
     v_scale: Optional[torch.Tensor] = None
 
 
-def _here(dev):
-    """The raw current stream of the current device, which `dev` has to be (the library launches on the current device)."""
-    if dev.type != "cuda":
+def _here(t):
+    """(device index, raw current stream) of the current device, on which `t` has to be (the library launches on the current device)."""
+    i = t.get_device()
+    if i < 0:
         raise L.Vlt5Error("tensor must be on the GPU")
-    i = torch._C._cuda_getDevice()
-    if dev.index != i:
-        raise L.Vlt5Error(f"tensor on {dev}, but cuda:{i} is the current device")
-    return torch._C._cuda_getCurrentRawStream(i)
+    if i != torch._C._cuda_getDevice():
+        raise L.Vlt5Error(f"tensor on {t.device}, but cuda:{torch._C._cuda_getDevice()} is the current device")
+    return i, torch._C._cuda_getCurrentRawStream(i)
 
 
 def _refuse(dev, *want):
@@ -411,7 +411,7 @@ def _row_stride(t, rows, cols):
 def quant_w4(w, group=128):
     """A weight [N, K] (f32 or bf16, unit column stride, K a multiple of 32) as a `W4Weight`."""
     dev = w.device
-    st = _here(dev)
+    _, st = _here(w)
     if w.dim() != 2 or w.dtype not in (BF16, torch.float32) or w.stride(1) != 1:
         _refuse(dev, ("w", w, (BF16, torch.float32), (None, None), False))
     N, K = w.shape
@@ -430,15 +430,15 @@ def decode_linear_w4(x, w, *, alpha=1.0, resid=None, relu=False, out_f32=False, 
     with out_f32; `out` takes the result instead (its type decides; it may be `resid` itself)."""
     codes, scales, group = w
     dev = x.device
-    st = _here(dev)
+    at, st = _here(x)
     if group not in (32, 64, 128):
         raise L.Vlt5Error(f"group: 32, 64 or 128, got {group}")
     if x.dim() != 2 or codes.dim() != 2:
         _refuse(dev, ("x", x, (BF16,), (None, None), False), ("codes", codes, (torch.uint8,), (None, None), True))
     (rows, K), (N, K2) = x.shape, codes.shape
     groups = -(-K // group)
-    if (x.dtype is not BF16 or x.stride(1) != 1 or K != 2 * K2 or codes.dtype is not torch.uint8 or codes.device != dev or not codes.is_contiguous()
-            or scales.dtype is not BF16 or scales.device != dev or scales.shape != (N, groups) or not scales.is_contiguous()):
+    if (x.dtype is not BF16 or x.stride(1) != 1 or K != 2 * K2 or codes.dtype is not torch.uint8 or codes.get_device() != at or not codes.is_contiguous()
+            or scales.dtype is not BF16 or scales.get_device() != at or scales.shape != (N, groups) or not scales.is_contiguous()):
         _refuse(dev, ("x", x, (BF16,), (None, 2 * K2), False), ("codes", codes, (torch.uint8,), (N, K2), True), ("scales", scales, (BF16,), (N, groups), True))
     if out is None:
         out = torch.empty(rows, N, device=dev, dtype=torch.float32 if out_f32 else BF16)
@@ -472,25 +472,26 @@ def kv_pages(n_pages, n_kv_heads, d_kv, page_size=64, dtype=torch.int8, device="
     return KVPages(k, v, *(torch.zeros(shape[:3], device=device, dtype=torch.float32) for _ in range(2)))
 
 
-def _paged(cache, table, kv_lens, cu_q, n_tok, max_q, dev):
+def _paged(cache, table, kv_lens, cu_q, n_tok, max_q, at, dev):
     """The cache and the sequences of a call as the library takes them."""
     k, v, ks, vs = cache
-    kind = _KV_TYPE.get(k.dtype)
+    dtype = k.dtype
+    kind = _KV_TYPE.get(dtype)
     if kind is None or k.dim() != 4 or table.dim() != 2:
         _refuse(dev, ("cache.k", k, tuple(_KV_TYPE), (None,) * 4, True), ("block table", table, (torch.int32,), (None, None), True))
     shape = k.shape
     B, mp = table.shape
-    if v.dtype is not k.dtype or v.shape != shape or v.device != dev or not k.is_contiguous() or not v.is_contiguous():
-        _refuse(dev, ("cache.k", k, (k.dtype,), tuple(shape), True), ("cache.v", v, (k.dtype,), tuple(shape), True))
+    if v.dtype is not dtype or v.shape != shape or k.get_device() != at or v.get_device() != at or not k.is_contiguous() or not v.is_contiguous():
+        _refuse(dev, ("cache.k", k, (dtype,), tuple(shape), True), ("cache.v", v, (dtype,), tuple(shape), True))
     n, h, page, d = shape
     ksp = vsp = None
     if kind:
         rows = (n, h, page)
-        if (ks is None or vs is None or ks.dtype is not torch.float32 or vs.dtype is not torch.float32 or ks.shape != rows or vs.shape != rows or ks.device != dev
-                or vs.device != dev or not ks.is_contiguous() or not vs.is_contiguous()):
+        if (ks is None or vs is None or ks.dtype is not F32 or vs.dtype is not F32 or ks.shape != rows or vs.shape != rows or ks.get_device() != at
+                or vs.get_device() != at or not ks.is_contiguous() or not vs.is_contiguous()):
             _refuse(dev, ("cache.k_scale", ks, (torch.float32,), rows, True), ("cache.v_scale", vs, (torch.float32,), rows, True))
         ksp, vsp = ks.data_ptr(), vs.data_ptr()
-    if (table.dtype is not torch.int32 or table.device != dev or not table.is_contiguous() or kv_lens.dtype is not torch.int32 or kv_lens.device != dev
+    if (table.dtype is not I32 or table.get_device() != at or not table.is_contiguous() or kv_lens.dtype is not I32 or kv_lens.get_device() != at
             or kv_lens.shape != (B,) or not kv_lens.is_contiguous()):
         _refuse(dev, ("block table", table, (torch.int32,), (B, mp), True), ("kv_lens", kv_lens, (torch.int32,), (B,), True))
     cu = None
@@ -499,7 +500,7 @@ def _paged(cache, table, kv_lens, cu_q, n_tok, max_q, dev):
         if n_tok != B and n_tok:
             raise L.Vlt5Error(f"{n_tok} tokens for {B} sequences: without cu_q every sequence has one")
     else:
-        if cu_q.dtype is not torch.int32 or cu_q.device != dev or cu_q.shape != (B + 1,) or not cu_q.is_contiguous():
+        if cu_q.dtype is not I32 or cu_q.get_device() != at or cu_q.shape != (B + 1,) or not cu_q.is_contiguous():
             _refuse(dev, ("cu_q", cu_q, (torch.int32,), (B + 1,), True))
         cu = cu_q.data_ptr()
     return (L.PagedKV(k.data_ptr(), v.data_ptr(), ksp, vsp, n, h, d, page, kind), L.PagedSeqs(table.data_ptr(), kv_lens.data_ptr(), cu, B, mp, n_tok, max_q or 0),
@@ -512,12 +513,12 @@ def kv_page_write(cache, k, v, table, kv_lens, *, cu_q=None, max_q=None):
     table i32 [B, pages of a sequence], kv_lens i32 [B]: keys of every sequence with the new tokens counted; cu_q i32 [B + 1]: first new
     token of every sequence (None: one token each); max_q: the most new tokens any of them has.  A page id outside the cache = not there."""
     dev = k.device
-    st = _here(dev)
-    if k.dim() != 2 or cache.k.device != dev:
-        _refuse(dev, ("k", k, (BF16,), (None, None), False), ("cache.k", cache.k, tuple(_KV_TYPE), (None,) * 4, True))
+    at, st = _here(k)
+    if k.dim() != 2:
+        _refuse(dev, ("k", k, (BF16,), (None, None), False))
     n, width = k.shape
-    kv, seqs, h, d, _ = _paged(cache, table, kv_lens, cu_q, n, max_q, dev)
-    if k.dtype is not BF16 or v.dtype is not BF16 or width != h * d or v.shape != (n, width) or v.device != dev or k.stride(1) != 1 or v.stride(1) != 1:
+    kv, seqs, h, d, _ = _paged(cache, table, kv_lens, cu_q, n, max_q, at, dev)
+    if k.dtype is not BF16 or v.dtype is not BF16 or width != h * d or v.shape != (n, width) or v.get_device() != at or k.stride(1) != 1 or v.stride(1) != 1:
         _refuse(dev, ("k", k, (BF16,), (None, h * d), False), ("v", v, (BF16,), (n, h * d), False))
     if n:
         check(lib().vlt5_kv_page_write(C.byref(kv), C.byref(seqs), k.data_ptr(), _row_stride(k, n, width), v.data_ptr(), _row_stride(v, n, width), st), "vlt5_kv_page_write")
@@ -526,8 +527,8 @@ def kv_page_write(cache, k, v, table, kv_lens, *, cu_q=None, max_q=None):
 def kv_page_read(cache, table, kv_lens, T):
     """Positions 0 .. T-1 of every sequence back as (k, v) bf16 [B, T, kv heads * d_kv], zeros at and past its length: what `attn_fwd` takes."""
     dev = cache.k.device
-    st = _here(dev)
-    kv, seqs, h, d, B = _paged(cache, table, kv_lens, None, 0, None, dev)
+    at, st = _here(cache.k)
+    kv, seqs, h, d, B = _paged(cache, table, kv_lens, None, 0, None, at, dev)
     k = torch.empty(B, T, h * d, device=dev, dtype=BF16)
     v = torch.empty(B, T, h * d, device=dev, dtype=BF16)
     if T:
@@ -544,11 +545,11 @@ def paged_attn(q, cache, table, kv_lens, *, cu_q=None, max_q=None, max_kv=None, 
     of the work only.  A token that sees no key gets zeros; rows of `out` that belong to no sequence keep what they hold.
     Returns out bf16 [tokens, heads * d_kv], with want_lse also f32 [tokens, heads] (-inf without keys)."""
     dev = q.device
-    st = _here(dev)
-    if q.dim() != 2 or cache.k.device != dev:
-        _refuse(dev, ("q", q, (BF16,), (None, None), False), ("cache.k", cache.k, tuple(_KV_TYPE), (None,) * 4, True))
+    at, st = _here(q)
+    if q.dim() != 2:
+        _refuse(dev, ("q", q, (BF16,), (None, None), False))
     n, width = q.shape
-    kv, seqs, h, d, _ = _paged(cache, table, kv_lens, cu_q, n, max_q, dev)
+    kv, seqs, h, d, _ = _paged(cache, table, kv_lens, cu_q, n, max_q, at, dev)
     if q.dtype is not BF16 or width % (h * d) or not width or q.stride(1) != 1:
         raise L.Vlt5Error(f"q: expected bf16 rows of a multiple of {h} heads of {d}, got {q.dtype} {tuple(q.shape)} with strides {tuple(q.stride())}")
     H = width // d
@@ -570,9 +571,10 @@ def paged_attn(q, cache, table, kv_lens, *, cu_q=None, max_q=None, max_kv=None, 
         desc = L.PagedAttnDesc(kv, seqs, q.data_ptr(), _row_stride(q, n, width), out.data_ptr(), o_st, None if lse is None else lse.data_ptr(), bias, nd, H, scale,
                                causal, max_kv or 0, None, 0)
         ref = C.byref(desc)
-        need = l.vlt5_paged_attn_workspace_bytes(ref)
-        if need > 0:
-            ws = torch.empty(need, device=dev, dtype=torch.uint8)
-            desc.workspace, desc.workspace_bytes = ws.data_ptr(), need
+        if (max_kv or seqs.max_pages * kv.page_size) >= L.PAGED_SHARED_KV:           # (below, the keys of a row are not shared out)
+            need = l.vlt5_paged_attn_workspace_bytes(ref)
+            if need > 0:
+                ws = torch.empty(need, device=dev, dtype=torch.uint8)
+                desc.workspace, desc.workspace_bytes = ws.data_ptr(), need
         check(l.vlt5_paged_attn(ref, st), "vlt5_paged_attn")
     return (out, lse) if want_lse else out
