@@ -645,16 +645,25 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
     float2 ml = make_float2(-INFINITY, 0.f);
     if (lane < a.splits) ml = *reinterpret_cast<const float2*>(a.part_ml + (lane * step + row) * 2);
     const int s0 = a.splits * part / WPR, s1 = a.splits * (part + 1) / WPR;
-    float acc[VEC] = {};
+    constexpr int MOST = WPR == 4 ? 16 : 8;                                        // splits of a wave
+    float x[MOST][VEC], acc[VEC] = {};
+#pragma unroll
+    for (int j = 0; j < MOST; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) x[j][i] = a.part_o[(min(s0 + j, a.splits - 1) * step + row) * DK + lane * VEC + i];
+#pragma unroll
+    for (int j = 0; j < MOST; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) arrived(x[j][i]);                            // (else each is requested where it is used)
     const float mx = wave_max(ml.x), ms = mx == -INFINITY ? 0.f : mx;
     const float f = exp2_hw((ml.x - ms) * LOG2E);
     const float sum = wave_sum(ml.y * f);
-#pragma unroll 8
-    for (int sp = s0; sp < s1; ++sp) {
-        const float* src = a.part_o + (sp * step + row) * DK + lane * VEC;
-        const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), sp));
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] = fmaf(src[i], fs, acc[i]);
+    for (int j = 0; j < MOST; ++j) {
+        if (s0 + j >= s1) break;
+        const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s0 + j));
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = fmaf(x[j][i], fs, acc[i]);
     }
     if constexpr (WPR > 1) {
         __shared__ float so[WPR][DK];
