@@ -119,7 +119,7 @@ __global__ __launch_bounds__(512) void w4_kernel(const W4Args a, int KS) {
     const bf16_t* srow = a.scales + (size_t)min(n_tile + r16, a.N - 1) * a.groups;
     const bf16_t* xl = xs + min(r16, rows - 1) * ld;
     auto load_w = [&](int c) {                                                 // (a piece past the end of the row: any codes, x is zero there)
-        return *reinterpret_cast<const uint4*>(wrow + c * 64 + (c * 128 + lseg * 32 < a.K ? lseg * 16 : 0));
+        return *reinterpret_cast<const vlt5_u32x4_t*>(wrow + c * 64 + (c * 128 + lseg * 32 < a.K ? lseg * 16 : 0));
     };
     struct Scales { bf16_t v[GPC]; };
     auto load_s = [&](int c, int end) {                                        // of chunk c + kq
@@ -138,12 +138,14 @@ __global__ __launch_bounds__(512) void w4_kernel(const W4Args a, int KS) {
     for (int cs = 0; cs < chunks; cs += KS / 128) {
         const int cnt = min(KS / 128, chunks - cs);
         const int c0 = cs + cnt * kw / KW, c1 = cs + cnt * (kw + 1) / KW;
-        uint4 wr[U];
-        Scales sn;
+        vlt5_u32x4_t wr[U];
+        Scales sn[U / 4];
+        if (c0 < c1) {                                                         // on their way while x is staged
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (c0 + u < c1) wr[u] = load_w(c0 + u);                           // on their way while x is staged
-        if (c0 < c1) sn = load_s(c0, c1);
+            for (int u = 0; u < U; ++u) if (c0 + u < c1) wr[u] = load_w(c0 + u);
+#pragma unroll
+            for (int q = 0; q < U / 4; ++q) sn[q] = load_s(c0 + q * 4, c1);
+        }
         if (cs) __syncthreads();                                               // every wave is done with the slab before
         const int kmax = min(KS, a.K - cs * 128), pieces = (cnt * 128) / 8;
         for (int i0 = threadIdx.x; i0 < rows * pieces; i0 += 4 * 512) {
@@ -161,37 +163,54 @@ __global__ __launch_bounds__(512) void w4_kernel(const W4Args a, int KS) {
                 if (at[q] >= 0) *reinterpret_cast<uint4*>(xs + at[q]) = v[q];
         }
         __syncthreads();
-        for (int c = c0; c < c1; c += U) {
-            const Scales sc = sn;
-            if (c + U < c1) sn = load_s(c + U, c1);
+        // one chunk: its codes through this wave's KB of LDS into the operand's layout (LDS operations of a wave complete in order: only the
+        // compiler has to keep it), its scales from the lane group that has them
+        auto multiply = [&](int c, const vlt5_u32x4_t& codes, const Scales& sc, int from) {
+            __builtin_amdgcn_wave_barrier();
+            *reinterpret_cast<vlt5_u32x4_t*>(turn + lane * 16) = codes;
+            __builtin_amdgcn_wave_barrier();
+            uint32_t sp[(GPC + 1) / 2];
+            __builtin_memcpy(sp, &sc, sizeof sc);
+#pragma unroll
+            for (int i = 0; i < (GPC + 1) / 2; ++i) sp[i] = __builtin_amdgcn_ds_bpermute((from * 16 + r16) * 4, sp[i]);
+#pragma unroll
+            for (int gi = 0; gi < GPC; ++gi) {
+                // this lane's codes of the group: 4 * DW bytes at gi * G / 2 + kq * 4 * DW of the column's 64
+                const int byte = gi * (G / 2) + kq * (4 * DW);
+                const char* p = turn + r16 * 64 + (((byte >> 4) ^ (r16 >> 2)) << 4) + (byte & 15);
+                uint32_t cw[DW];
+                __builtin_memcpy(cw, __builtin_assume_aligned(p, 4 * DW), sizeof cw);
+                f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < DW; ++e) {
+                    const bf16x8_t fx = *reinterpret_cast<const bf16x8_t*>(xl + (c - cs) * 128 + gi * G + kq * (8 * DW) + e * 8);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx, fp4x8(cw[e]), acc, 0, 0, 0);
+                }
+                const float s = __uint_as_float(gi & 1 ? sp[gi / 2] & 0xffff0000u : sp[gi / 2] << 16);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) tot[r] = fmaf(s, acc[r], tot[r]);
+            }
+        };
+        int c = c0;
+        for (; c + 2 * U <= c1; c += U) {                                      // (every load unconditional, or the waits could not be counted)
+            Scales sc[U / 4];
+#pragma unroll
+            for (int q = 0; q < U / 4; ++q) { sc[q] = sn[q]; sn[q] = load_s(c + U + q * 4, c1); }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                multiply(c + u, wr[u], sc[u / 4], u % 4);
+                wr[u] = load_w(c + u + U);
+            }
+        }
+        for (; c < c1; c += U) {
+            Scales sc[U / 4];
+#pragma unroll
+            for (int q = 0; q < U / 4; ++q) { sc[q] = sn[q]; if (c + U < c1) sn[q] = load_s(c + U + q * 4, c1); }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (c + u >= c1) break;
-                __builtin_amdgcn_wave_barrier();                               // (LDS operations of one wave complete in order: only the compiler has to keep it)
-                *reinterpret_cast<uint4*>(turn + lane * 16) = wr[u];
-                __builtin_amdgcn_wave_barrier();
+                multiply(c + u, wr[u], sc[u / 4], u % 4);
                 if (c + u + U < c1) wr[u] = load_w(c + u + U);
-                uint32_t sp[(GPC + 1) / 2];
-                __builtin_memcpy(sp, &sc, sizeof sc);
-#pragma unroll
-                for (int i = 0; i < (GPC + 1) / 2; ++i) sp[i] = __builtin_amdgcn_ds_bpermute((u * 16 + r16) * 4, sp[i]);
-#pragma unroll
-                for (int gi = 0; gi < GPC; ++gi) {
-                    // this lane's codes of the group: 4 * DW bytes at gi * G / 2 + kq * 4 * DW of the column's 64
-                    const int byte = gi * (G / 2) + kq * (4 * DW);
-                    const char* p = turn + r16 * 64 + (((byte >> 4) ^ (r16 >> 2)) << 4) + (byte & 15);
-                    uint32_t cw[DW];
-                    __builtin_memcpy(cw, __builtin_assume_aligned(p, 4 * DW), sizeof cw);
-                    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int e = 0; e < DW; ++e) {
-                        const bf16x8_t fx = *reinterpret_cast<const bf16x8_t*>(xl + (c + u - cs) * 128 + gi * G + kq * (8 * DW) + e * 8);
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx, fp4x8(cw[e]), acc, 0, 0, 0);
-                    }
-                    const float s = __uint_as_float(gi & 1 ? sp[gi / 2] & 0xffff0000u : sp[gi / 2] << 16);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) tot[r] = fmaf(s, acc[r], tot[r]);
-                }
             }
         }
     }
