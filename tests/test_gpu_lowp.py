@@ -551,3 +551,132 @@ def test_refusals(dev, ops):
     assert ops.paged_attn(q[:0], c, t, n, cu_q=ints(dev, [0, 0, 0])).shape == (0, 256)
     k, v = ops.kv_page_read(c, t, n, 0)
     assert k.shape == v.shape == (2, 0, 128)
+
+
+# ---- the corners of a call --------------------------------------------------------------------------------------------------------
+def test_decode_linear_w4_slabs_with_a_short_end(dev, ops):
+    """Rows of x that do not fit LDS, of a length that is no multiple of 128 or of the group; extreme values beside zeros."""
+    for rows, N, K, group in ((16, 40, 11040, 128), (13, 17, 9952, 64), (16, 20, 4736, 32)):
+        g = gen(K)
+        w = ops.quant_w4((torch.randn(N, K, generator=g) * K ** -0.5).to(dev), group)
+        x = torch.randn(rows, K, generator=g).to(BF)
+        x[0] = 0
+        x[1, ::7] *= 1e4
+        v = w4_value(w)
+        y = ops.decode_linear_w4(x.to(dev), w, out_f32=True).cpu().double()
+        ref = x.double() @ v.t()
+        assert bool(((y - ref).abs() <= (group + -(-K // group) + 16) * U * (x.double().abs() @ v.abs().t())).all())
+        assert bool((y[0] == 0).all())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_more_new_tokens_than_keys(dev, ops, kind):
+    """Positions below zero: nothing is written for them, they see nothing; the others are as ever."""
+    lens, new = [3, 40], [7, 2]
+    c, table = make_cache(ops, dev, [16, 48], 2, 64, 16, kind, seed=31)
+    before = [None if t is None else raw(t).cpu().clone() for t in c]
+    x = torch.randn(9, 128, generator=gen(3)).to(BF).to(dev)
+    args = (table.to(dev), ints(dev, lens))
+    ops.kv_page_write(c, x, x, *args, cu_q=ints(dev, starts(new)))
+    codes, sc = plain_codes(x.cpu().view(9, 2, 64), kind)
+    p = int(table[0, 0])
+    assert torch.equal(raw(c.k)[p, :, :3].cpu(), raw(codes)[4:7].transpose(0, 1)) and torch.equal(raw(c.k)[p, :, 3:].cpu(), before[0][p, :, 3:])
+    out, lse = ops.paged_attn(x, c, *args, cu_q=ints(dev, starts(new)), want_lse=True)
+    assert bool((out[:4] == 0).all()) and bool((lse[:4] == -math.inf).all())
+    ref, tol, _ = attn_ref(x[4:].cpu(), c, table, [3, 2], lens, 2, 1.0, True, None)
+    assert bool(((out[4:].cpu().double().view(5, 2, 64) - ref).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("new", [[3, 9], [90, 40]])
+def test_max_q_limits_what_is_processed(dev, ops, new):
+    """Tokens past max_q are left alone by the write and by the attention."""
+    lens = [100, 60]
+    c, table = make_cache(ops, dev, lens, 2, 64, 16, torch.int8, seed=32)
+    n, most = sum(new), min(new)
+    x = torch.randn(n, 128, generator=gen(4)).to(BF).to(dev)
+    args = (table.to(dev), ints(dev, lens))
+    full = ops.paged_attn(x, c, *args, cu_q=ints(dev, starts(new)))
+    out = torch.full((n, 128), 3.0, device=dev, dtype=BF)
+    ops.paged_attn(x, c, *args, cu_q=ints(dev, starts(new)), max_q=most, out=out)
+    for b in range(2):
+        s = starts(new)[b]
+        assert bool((out[s + most: s + new[b]] == 3.0).all())
+        ref, tol, _ = attn_ref(x.cpu(), c, table, new, lens, 2, 1.0, True, None)
+        err = (out[s: s + most].cpu().double().view(-1, 2, 64) - ref[s: s + most]).abs()
+        assert bool((err <= tol[s: s + most]).all())
+    assert full.shape == out.shape
+    before = raw(c.k).clone()
+    ops.kv_page_write(c, x, x, *args, cu_q=ints(dev, starts(new)), max_q=1)
+    changed = (raw(c.k) != before).any(-1).nonzero().cpu()
+    want = {(int(table[b, (lens[b] - new[b]) // 16]), (lens[b] - new[b]) % 16) for b in range(2)}
+    assert {(int(p), int(r)) for p, _, r in changed} == want
+
+
+def test_strided_rows_and_shared_pages(dev, ops):
+    """q, k, v and out as slices of wider buffers; two sequences that share the pages of a prefix; out in the place of q."""
+    c, _ = make_cache(ops, dev, [96, 96], 2, 64, 16, FP8, seed=33)
+    table = torch.tensor([[0, 1, 2, 3], [0, 1, 4, 5]], dtype=torch.int32)                  # 32 positions in common
+    lens, new = [50, 60], [5, 20]
+    wide = torch.randn(25, 904, generator=gen(5)).to(BF).to(dev)
+    q, k, v = wide[:, 8:264], wide[:, 264:392], wide[:, 400:528]
+    args = (table.to(dev), ints(dev, lens))
+    ops.kv_page_write(c, k, v, *args, cu_q=ints(dev, starts(new)))
+    kr, _ = ops.kv_page_read(c, *args, 64)
+    kk, _ = held(c, table, 1, 60)
+    assert torch.equal(kr[1, :60].cpu().double(), kk.flatten(1).float().to(BF).double()) and torch.equal(kr[0, :32], kr[1, :32])
+    buf = torch.full((25, 304), 2.0, device=dev, dtype=BF)
+    out = ops.paged_attn(q, c, *args, cu_q=ints(dev, starts(new)), out=buf[:, 16:272])
+    ref, tol, _ = attn_ref(q.cpu(), c, table, new, lens, 4, 1.0, True, None)
+    assert bool(((out.cpu().double().view(25, 4, 64) - ref).abs() <= tol).all())
+    assert bool((buf[:, :16] == 2).all()) and bool((buf[:, 272:] == 2).all())
+    mine = q.contiguous()
+    assert torch.equal(ops.paged_attn(mine, c, *args, cu_q=ints(dev, starts(new)), out=mine), out) and torch.equal(mine, out)
+    from vqacl_amd._lib import Vlt5Error
+    for bad in (lambda: ops.paged_attn(wide[:, 4:260], c, *args, cu_q=ints(dev, starts(new))), lambda: ops.kv_page_write(c, wide[:, 4:132], v, *args, cu_q=ints(dev, starts(new))),
+                lambda: ops.paged_attn(q, c, *args, cu_q=ints(dev, starts(new)), scale=0.0), lambda: ops.paged_attn(q, c, *args, cu_q=ints(dev, starts(new)), scale=-1.0)):
+        with pytest.raises(Vlt5Error):
+            bad()
+
+
+@pytest.mark.parametrize("scale", [1e-39, 1e-30, 30.0])
+@pytest.mark.parametrize("new", [1, 40])
+def test_extreme_scales(dev, ops, scale, new):
+    """All keys alike, and one key alone: the running maximum's slack follows the scale."""
+    lens = [300]
+    c, table = make_cache(ops, dev, lens, 2, 64, 16, torch.int8, seed=34)
+    check_attn(ops, dev, c, table, [new], lens, 4, scale=scale, seed=1)
+
+
+@pytest.mark.parametrize("kind", [torch.int8, FP8])
+def test_a_token_that_is_not_finite_is_seen_by_later_ones_only(dev, ops, kind):
+    """8-bit types: a NaN or an infinity in a new token's key or value shows in the tokens that see it and in no other."""
+    new, lens = [70], [90]
+    c, table = make_cache(ops, dev, lens, 1, 64, 16, kind, seed=35)
+    x = torch.randn(70, 64, generator=gen(6)).to(BF)
+    x[41, 5], x[41, 6] = math.nan, math.inf
+    for k, v in ((x, x.nan_to_num(0, 0, 0)), (x.nan_to_num(0, 0, 0), x)):
+        ops.kv_page_write(c, k.to(dev), v.to(dev), table.to(dev), ints(dev, lens), cu_q=ints(dev, [0, 70]))
+        for heads in (1, 4):                                                               # through both kernels
+            out = ops.paged_attn(torch.ones(70, 64 * heads, device=dev, dtype=BF), c, table.to(dev), ints(dev, lens), cu_q=ints(dev, [0, 70]), scale=0.1)
+            assert bool(torch.isfinite(out[:41]).all()) and bool(torch.isnan(out[41:]).all())
+
+
+def test_a_cold_call_inside_a_capture_and_two_graphs(dev, ops):
+    """Two graphs of the same step, replayed in turn and with eager calls between: each has a workspace of its own."""
+    lens = [6000]
+    c, table = make_cache(ops, dev, lens, 4, 128, 64, FP8, seed=36)
+    t, n = table.to(dev), ints(dev, lens)
+    qs = [torch.randn(1, 16 * 128, generator=gen(50 + i)).to(BF).to(dev) for i in range(3)]
+    want = [ops.paged_attn(q, c, t, n, scale=0.09) for q in qs]
+    graphs = []
+    for q in qs[:2]:
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = ops.paged_attn(q, c, t, n, scale=0.09)
+        graphs.append((g, y))
+    for i in (0, 1, 1, 0, 1):
+        graphs[i][0].replay()
+        assert torch.equal(ops.paged_attn(qs[2], c, t, n, scale=0.09), want[2])
+        torch.cuda.synchronize()
+        assert torch.equal(graphs[i][1], want[i])

@@ -12,6 +12,10 @@ struct PagedSeqs {
     int B, n_tok, max_q;
 };
 
+// csrc/paged.hip: host-side checks shared by the entry points of the cache, and the kernels' view of a call
+int vlt5_paged_check(const vlt5_paged_kv* c, const vlt5_paged_seqs* q);
+PagedSeqs vlt5_paged_seqs_of(const vlt5_paged_kv* c, const vlt5_paged_seqs* q);
+
 struct PagedSeq {
     int q0, nq, len;          // first new token, number of new tokens, keys (new ones included)
 };

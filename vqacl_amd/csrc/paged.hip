@@ -152,7 +152,6 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const PagedSeqs s, const u
 
 }  // namespace
 
-// host-side checks shared by the entry points of the cache
 int vlt5_paged_check(const vlt5_paged_kv* c, const vlt5_paged_seqs* q) {
     if (!c || !q || !c->k || !c->v || !q->table || !q->kv_lens) return VLT5_ERR_ARG;
     if (c->type != VLT5_KV_BF16 && c->type != VLT5_KV_INT8 && c->type != VLT5_KV_FP8) return VLT5_ERR_ARG;

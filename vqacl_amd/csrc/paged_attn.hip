@@ -1,14 +1,19 @@
 // Attention of the newest tokens of every sequence over its paged cache: softmax(scale * q K^T + bias) V, single tokens and chunks.
 //
-// The query rows of one (sequence, kv head) are the tokens times the query heads that share the kv head, sixteen of them a tile.  Keys are
-// walked in tiles of 64 with the running maximum and sum of the softmax in f32, and everything stays in registers:
-//   scores  S^T[key, row] = mfma(A = 16 keys, B = 16 query rows): a lane ends up with four consecutive keys of ONE row (row = lane % 16);
-//   output  O^T[d, row] += mfma(A = V^T, B = P^T): the 32 keys of one instruction may be taken in any order as long as both operands agree,
-//           so the eight keys of a lane's B operand are simply the ones it has scores of -- no exchange between lanes -- and the A operand is
-//           built from the same eight rows of V, d_kv / 16 neighbouring values of each: the conversion to bf16 pairs them by key, which IS
-//           the transposition.
+// The query rows of one (sequence, kv head) are the tokens times the query heads that share the kv head.  Few rows (paged_attn_kernel): sixteen
+// a tile, every wave for itself, everything in registers.  Many rows (paged_chunk_kernel): 128 a workgroup, keys and values converted to bf16
+// once and shared through LDS.  In both, with the running maximum and sum of the softmax in f32:
+//   scores  S^T[key, row] = mfma(A = keys, B = query rows): a lane ends up with runs of four consecutive keys of ONE row;
+//   output  O^T[d, row] += mfma(A = V^T, B = P^T): the keys of one instruction may be taken in any order as long as both operands agree, so
+//           the eight keys of a lane's B operand are simply ones it has scores of -- no exchange between lanes -- and the A operand is built
+//           from the same eight rows of V, a few neighbouring values of each: the conversion to bf16 pairs them by key, which IS the
+//           transposition.
 // 8-bit codes are exact in bf16; the scale of a key multiplies its score, the scale of a value its probability (in f32, before the one
-// rounding of the probabilities to bf16).
+// rounding of the probabilities to bf16, which with the output's own is all the rounding there is below 32 bits).
+//
+// Single tokens are bound by the bytes of the cache: 32 x 16384 keys, 8 kv heads of 128, e4m3: 148 us = 5.5 TB/s; 1 x 131071, int8: 42 us =
+// 6.6 TB/s (a part of it from the last-level cache) and 4.6 us to join its 64 shares.  Long chunks are bound by the matrix and vector units
+// together (42 % and 41 % busy at the 1.8 GHz such a load runs at): 2048 tokens over 16384 bf16 keys, 32 heads of 128: 570-590 us = 890 TFLOP/s.
 #include "paged.h"
 
 namespace {
@@ -126,7 +131,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_kernel(const PagedAttnA
     float bias_far = bias ? bias[a.nd - 1] : 0.f;
     arrived(bias_far);
     // scores and their maximum are kept as q k (times the key's scale), with a bias as scale * q k + bias; `unit` makes powers of two of them
-    const float unit = bias ? LOG2E : a.scale * LOG2E, lag = 8.f / unit;
+    const float unit = bias ? LOG2E : a.scale * LOG2E, lag = fminf(8.f / unit, 1e38f);
 
     f32x4_t o[ND];
 #pragma unroll
@@ -364,12 +369,13 @@ __global__ __launch_bounds__(256 * KS, 2) void paged_chunk_kernel(const PagedAtt
     if (near_lds)
         for (int i = tid; i < a.g * a.nd; i += 256 * KS) sb[i] = a.bias[(size_t)hk * a.g * a.nd + i];      // (the barrier before the first tile covers it)
     // scores and their maximum are kept as q k (times the key's scale), with a bias as scale * q k + bias; `unit` makes powers of two of them
-    const float unit = BIAS ? LOG2E : a.scale * LOG2E, lag = 8.f / unit;
+    const float unit = BIAS ? LOG2E : a.scale * LOG2E, lag = fminf(8.f / unit, 1e38f);
 
     // ---- one tile's raw rows on their way ----
     vlt5_u32x4_t kr[KP];
     uint32_t vr[8][VW];
-    float scl = 0.f;
+    float ksc = 0.f, vsc = 0.f;
+    bool sees = false;
     // the keys of 16 are in one page; lane j: page of the j-th 16 keys of the 16 tiles from (tile & ~15) on, or -1
     int ids = -1, pg[4], pn[4];                                                         // ... and those of this tile and the next
     const int tiles = (hi - lo + 63) / 64;
@@ -400,11 +406,12 @@ __global__ __launch_bounds__(256 * KS, 2) void paged_chunk_kernel(const PagedAtt
             else vr[e][0] = *reinterpret_cast<const uint16_t*>(p);
         }
         if constexpr (KvType<T>::SCALED) {
-            const bool ws = w4 == 1;                                                    // wave 0: key scales, wave 1: value scales
-            if (w4 < 2) {
+            if (w4 == 0) {
                 const int page = lane < 16 ? pn[0] : (lane < 32 ? pn[1] : (lane < 48 ? pn[2] : pn[3]));
-                scl = (ws ? a.vs : a.ks)[first_row(page, t0 + lane)];
-                if (ws && (page < 0 || t0 + lane >= sq.len)) scl = 0.f;
+                const size_t at = first_row(page, t0 + lane);
+                ksc = a.ks[at];
+                vsc = a.vs[at];
+                sees = page >= 0 && t0 + lane < sq.len;
             }
         }
         // what lies behind the last key or in a page that is not there may hold anything, NaN too
@@ -442,7 +449,12 @@ __global__ __launch_bounds__(256 * KS, 2) void paged_chunk_kernel(const PagedAtt
             *reinterpret_cast<uint4*>(v + ((w4 * NT + j) * 64 + lane) * 16) = make_uint4(q[0], q[1], q[2], q[3]);
         }
         if constexpr (KvType<T>::SCALED)
-            if (w4 < 2) reinterpret_cast<float*>(v + VBYTES)[w4 * 64 + lane] = scl;
+            if (w4 == 0) {
+                // a value scale that is not finite moves to the key's side: a masked score is dropped, but a masked probability of 0 times it is not 0
+                const bool fine = fabsf(vsc) <= 3.402823466e38f;
+                reinterpret_cast<float*>(v + VBYTES)[lane] = fine ? ksc : __uint_as_float(0x7fc00000u);
+                reinterpret_cast<float*>(v + VBYTES)[64 + lane] = fine && sees ? vsc : 0.f;
+            }
     };
 
     f32x16_t o[NT];
@@ -698,6 +710,10 @@ int chunk_launch(const PagedAttnArgs& a, unsigned blocks, hipStream_t st) {
 // 100 x 500: 20.4 against 19.1), and by as many workgroups as give every CU two, none with less than 512 keys (1 x 131071 keys, 8 kv heads of 128,
 // int8: 67 us in 64 shares; 8 x 2000 keys: 15 us in 3 shares of 667, 17 in 7 of 286).  Large tiles that leave a CU one workgroup get twice the
 // waves, half the keys each (8 sequences of 200 tokens over 712 keys, 12 heads: 28.4 -> 20.5 us; where CUs have two anyway it costs 5 %).
+// query heads a multiple of the kv heads; rows are counted in 32 bits
+bool paged_heads_ok(const vlt5_paged_attn_desc* d) {
+    return d->H > 0 && d->H <= 1024 && d->H % d->kv.n_kv_heads == 0 && (long long)d->seqs.n_tok * d->H <= 0x7fffffffLL - 4096;
+}
 struct PagedPlan { int chunk, row_tiles, splits, waves; };
 PagedPlan paged_plan(const vlt5_paged_attn_desc* d, const PagedSeqs& s) {
     const int g = d->H / d->kv.n_kv_heads;
@@ -717,11 +733,8 @@ PagedPlan paged_plan(const vlt5_paged_attn_desc* d, const PagedSeqs& s) {
 
 }  // namespace
 
-int vlt5_paged_check(const vlt5_paged_kv* c, const vlt5_paged_seqs* q);
-PagedSeqs vlt5_paged_seqs_of(const vlt5_paged_kv* c, const vlt5_paged_seqs* q);
-
 extern "C" long long vlt5_paged_attn_workspace_bytes(const vlt5_paged_attn_desc* d) {
-    if (!d || vlt5_paged_check(&d->kv, &d->seqs) || d->H <= 0 || d->H % d->kv.n_kv_heads) return -1;
+    if (!d || vlt5_paged_check(&d->kv, &d->seqs) || !paged_heads_ok(d)) return -1;
     const PagedSeqs s = vlt5_paged_seqs_of(&d->kv, &d->seqs);
     const int sp = paged_plan(d, s).splits;
     return sp == 1 ? 0 : (long long)sp * s.n_tok * d->H * (d->kv.d_kv + 2) * 4;
@@ -732,7 +745,7 @@ extern "C" int vlt5_paged_attn(const vlt5_paged_attn_desc* d, void* stream) {
     const int rc = vlt5_paged_check(&d->kv, &d->seqs);
     if (rc) return rc;
     const vlt5_paged_kv& c = d->kv;
-    if (d->H <= 0 || d->H % c.n_kv_heads || d->H > 1024) return VLT5_ERR_ARG;
+    if (!paged_heads_ok(d)) return VLT5_ERR_ARG;
     if (d->q_st < (long long)d->H * c.d_kv || d->o_st < (long long)d->H * c.d_kv) return VLT5_ERR_ARG;
     if (d->rel_bias && (d->n_dist <= 0 || !d->causal)) return VLT5_ERR_ARG;
     if (!(d->scale > 0.f && d->scale <= 3.402823466e38f)) return VLT5_ERR_ARG;
