@@ -686,8 +686,11 @@ int vlt5_decode_attn(const vlt5_attn_desc* d, void* stream);
  * nearest e2m1 number to w / scale (f32, ties to the even code); a group with an infinity or a NaN gets the scale NaN. */
 int vlt5_quant_w4(const float* w_f32, const void* w_bf16, long long ldw, int N, int K, int group, void* codes, void* scales, void* stream);
 /* out[m, n] = act(alpha * sum_k x[m, k] value(code[n, k]) scale[n, k / group] (+ resid[m, n])), the vlt5_decode_linear of such a weight:
- * rows <= VLT5_W4_MAX_ROWS, any N, x bf16 (rows 16-byte aligned), f32 sums, bf16 and / or f32 output.  `resid` may be `out_f32`. */
+ * rows <= VLT5_W4_MAX_ROWS, any N, x bf16 (rows 16-byte aligned), f32 sums, bf16 and / or f32 output.  `resid` may be `out_f32`.
+ * workspace: vlt5_decode_linear_w4_workspace_bytes (0: none needed, always so where 2 * min(rows, 16) * K < VLT5_W4_SPLIT_BYTES), 16-byte
+ * aligned, one per call in flight. */
 #define VLT5_W4_MAX_ROWS 256
+#define VLT5_W4_SPLIT_BYTES 131072
 typedef struct {
     const void* x_bf16; long long ldx;
     const void* codes; const void* scales; int rows, N, K, group;
@@ -696,7 +699,9 @@ typedef struct {
     float* out_f32; long long ld_out_f32;
     const float* resid; long long ld_resid;
     int relu;
+    void* workspace; long long workspace_bytes;
 } vlt5_decode_linear_w4_desc;
+long long vlt5_decode_linear_w4_workspace_bytes(int rows, int N, int K);
 int vlt5_decode_linear_w4(const vlt5_decode_linear_w4_desc* d, void* stream);
 
 /* The cache of one layer.  k, v: [n_pages][n_kv_heads][page_size][d_kv] of bf16, int8 or e4m3; k_scale, v_scale: f32

@@ -556,7 +556,9 @@ def test_refusals(dev, ops):
 # ---- the corners of a call --------------------------------------------------------------------------------------------------------
 def test_decode_linear_w4_slabs_with_a_short_end(dev, ops):
     """Rows of x that do not fit LDS, of a length that is no multiple of 128 or of the group; extreme values beside zeros."""
-    for rows, N, K, group in ((16, 40, 11040, 128), (13, 17, 9952, 64), (16, 20, 4736, 32)):
+    for rows, N, K, group, split in ((16, 40, 11040, 128, True), (13, 17, 9952, 64, True), (40, 100, 4640, 32, True), (16, 4112, 5152, 64, False), (100, 700, 5024, 32, False)):
+        from vqacl_amd._lib import lib
+        assert (lib().vlt5_decode_linear_w4_workspace_bytes(rows, N, K) > 0) == split      # slabs in workgroups of their own, or one after the other
         g = gen(K)
         w = ops.quant_w4((torch.randn(N, K, generator=g) * K ** -0.5).to(dev), group)
         x = torch.randn(rows, K, generator=g).to(BF)
@@ -565,8 +567,13 @@ def test_decode_linear_w4_slabs_with_a_short_end(dev, ops):
         v = w4_value(w)
         y = ops.decode_linear_w4(x.to(dev), w, out_f32=True).cpu().double()
         ref = x.double() @ v.t()
-        assert bool(((y - ref).abs() <= (group + -(-K // group) + 16) * U * (x.double().abs() @ v.abs().t())).all())
+        acc = (group + -(-K // group) + 16) * U * (x.double().abs() @ v.abs().t())
+        assert bool(((y - ref).abs() <= acc).all())
         assert bool((y[0] == 0).all())
+        resid = torch.randn(rows, N, generator=g).to(dev)
+        z = ops.decode_linear_w4(x.to(dev), w, alpha=0.5, relu=True, resid=resid, out=resid.to(BF)).cpu().double()
+        want = (0.5 * ref + resid.cpu().double()).clamp_min(0)
+        assert bool(((z - want).abs() <= acc + U * want + H * want).all())
 
 
 @pytest.mark.parametrize("kind", KINDS)

@@ -46,6 +46,17 @@ def test_w4_refusals(built):
                        ({"codes": P + 8}, ALIGN), ({"x_bf16": P + 2}, ALIGN)):
         d = built.DecodeLinearW4Desc(**{**ok, **change})
         assert f(C.byref(d), None) == rc, change
+    # long rows for few columns: the reduction is split and needs a workspace of its own
+    size = built.lib().vlt5_decode_linear_w4_workspace_bytes
+    long = dict(ok, rows=16, K=8192, ldx=8192)
+    need = size(16, 8, 8192)
+    assert need > 0 and need % (4 * 16 * 8) == 0
+    for change, rc in (({}, ARG), ({"workspace": P, "workspace_bytes": need - 1}, ARG), ({"workspace": P + 8, "workspace_bytes": need}, ALIGN)):
+        assert f(C.byref(built.DecodeLinearW4Desc(**{**long, **change})), None) == rc, change
+    edge = built.W4_SPLIT_BYTES
+    assert f"#define VLT5_W4_SPLIT_BYTES {edge}\n" in open(os.path.join(ROOT, "include", "vlt5_hip.h")).read()
+    assert size(16, 8, edge // 32 - 32) == 0 and size(16, 8, edge // 32) > 0 and size(1, 8, edge // 2) > 0 and size(16, 32200, 8192) == 0
+    assert size(0, 8, 64) == size(257, 8, 64) == size(4, 0, 64) == size(4, 8, 0) == -1
     q = built.lib().vlt5_quant_w4
     assert q(None, None, 64, 4, 64, 32, P, P, None) == ARG and q(P, P, 64, 4, 64, 32, P, P, None) == ARG and q(P, None, 64, 4, 64, 33, P, P, None) == ARG
     assert q(P, None, 64, 0, 64, 32, P, P, None) == ARG and q(P, None, 32, 4, 64, 32, P, P, None) == ARG and q(P, None, 64, 4, 64, 32, None, P, None) == ARG

@@ -178,7 +178,7 @@ class DecodeLinearDesc(C.Structure):
 class DecodeLinearW4Desc(C.Structure):
     _fields_ = [("x_bf16", vp), ("ldx", c_ll), ("codes", vp), ("scales", vp), ("rows", c_i), ("N", c_i), ("K", c_i), ("group", c_i),
                 ("alpha", c_f), ("out_bf16", vp), ("ld_out_bf16", c_ll), ("out_f32", vp), ("ld_out_f32", c_ll), ("resid", vp),
-                ("ld_resid", c_ll), ("relu", c_i)]
+                ("ld_resid", c_ll), ("relu", c_i), ("workspace", vp), ("workspace_bytes", c_ll)]
 
 
 class PagedKV(C.Structure):
@@ -294,6 +294,7 @@ PROTOTYPES = {
     "vlt5_decode_linear_tiles": (c_i, [c_i, c_i, c_i, c_i]),
     "vlt5_decode_attn": (c_i, [C.POINTER(AttnDesc), vp]),
     "vlt5_quant_w4": (c_i, [vp, vp, c_ll, c_i, c_i, c_i, vp, vp, vp]),
+    "vlt5_decode_linear_w4_workspace_bytes": (c_ll, [c_i, c_i, c_i]),
     "vlt5_decode_linear_w4": (c_i, [C.POINTER(DecodeLinearW4Desc), vp]),
     "vlt5_kv_page_write": (c_i, [C.POINTER(PagedKV), C.POINTER(PagedSeqs), vp, c_ll, vp, c_ll, vp]),
     "vlt5_kv_page_read": (c_i, [C.POINTER(PagedKV), C.POINTER(PagedSeqs), c_i, vp, vp, vp]),
@@ -306,6 +307,7 @@ PROTOTYPES = {
 WS_ENC_OUT, WS_ENC_EXT, WS_LOGITS, WS_LOSS_TOK, WS_LOSS, WS_ENC_MASK_EXT, WS_DEC_OUT = range(7)
 
 PAGED_SHARED_KV = 1024         # VLT5_PAGED_SHARED_KV
+W4_SPLIT_BYTES = 131072        # VLT5_W4_SPLIT_BYTES
 
 _lib = None
 ABI_VERSION = 8

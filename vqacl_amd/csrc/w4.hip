@@ -78,6 +78,7 @@ struct W4Args {
     float* out_f; long long ldf;
     const float* resid; long long ldr;
     int relu;
+    int splits; float* part;                   // > 1: the reduction in this many runs of chunks, their sums [splits][rows][N]
 };
 
 __device__ __forceinline__ void w4_store(const W4Args& a, int m, int n, float sum) {
@@ -134,8 +135,8 @@ __global__ __launch_bounds__(512) void w4_kernel(const W4Args a, int KS) {
         return s;
     };
     f32x4_t tot = {0.f, 0.f, 0.f, 0.f};
-    const int chunks = (a.K + 127) / 128;
-    for (int cs = 0; cs < chunks; cs += KS / 128) {
+    const int all = (a.K + 127) / 128, start = (int)((long long)all * blockIdx.z / a.splits), chunks = (int)((long long)all * (blockIdx.z + 1) / a.splits);
+    for (int cs = start; cs < chunks; cs += KS / 128) {
         const int cnt = min(KS / 128, chunks - cs);
         const int c0 = cs + cnt * kw / KW, c1 = cs + cnt * (kw + 1) / KW;
         vlt5_u32x4_t wr[U];
@@ -146,7 +147,7 @@ __global__ __launch_bounds__(512) void w4_kernel(const W4Args a, int KS) {
 #pragma unroll
             for (int q = 0; q < U / 4; ++q) sn[q] = load_s(c0 + q * 4, c1);
         }
-        if (cs) __syncthreads();                                               // every wave is done with the slab before
+        if (cs != start) __syncthreads();                                      // every wave is done with the slab before
         const int kmax = min(KS, a.K - cs * 128), pieces = (cnt * 128) / 8;
         for (int i0 = threadIdx.x; i0 < rows * pieces; i0 += 4 * 512) {
             uint4 v[4];
@@ -227,32 +228,61 @@ __global__ __launch_bounds__(512) void w4_kernel(const W4Args a, int KS) {
         }
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) w4_store(a, m_tile + kq * 4 + r, n_tile + r16, tot[r]);
+    for (int r = 0; r < 4; ++r) {
+        const int m = m_tile + kq * 4 + r, n = n_tile + r16;
+        if (a.splits == 1) w4_store(a, m, n, tot[r]);
+        else if (m < a.rows && n < a.N) a.part[((size_t)blockIdx.z * a.rows + m) * a.N + n] = tot[r];
+    }
+}
+
+// the runs of a split reduction, added in their order
+__global__ __launch_bounds__(256) void w4_join_kernel(const W4Args a) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, all = (long long)a.rows * a.N;
+    if (i >= all) return;
+    float s = 0.f;
+    for (int z = 0; z < a.splits; ++z) s += a.part[z * all + i];
+    w4_store(a, (int)(i / a.N), (int)(i % a.N), s);
 }
 
 template <int G, int KW>
 int w4_launch(const W4Args& a, hipStream_t st) {
     static std::atomic<unsigned long long> done{0};
     const int rows = a.rows < 16 ? a.rows : 16;
-    const int kpad = (a.K + 127) & ~127, room = 148 * 1024 / 2 / rows - 8;      // 8 KB of the 160 are for the codes on their way
-    const int KS = kpad <= room ? kpad : room & ~127;
+    const int run = ((a.K + 127) / 128 + a.splits - 1) / a.splits * 128, room = 148 * 1024 / 2 / rows - 8;      // 8 KB of the 160 are for the codes on their way
+    const int KS = run <= room ? run : room & ~127;
     const int rc = vlt5_lds_optin((const void*)w4_kernel<G, KW>, 160 * 1024, done);
     if (rc) return rc;
-    const dim3 grid(((a.N + 15) / 16 + 8 / KW - 1) / (8 / KW), (a.rows + 15) / 16);
+    const dim3 grid(((a.N + 15) / 16 + 8 / KW - 1) / (8 / KW), (a.rows + 15) / 16, a.splits);
     hipLaunchKernelGGL((w4_kernel<G, KW>), grid, dim3(512), 8 * 1024 + rows * (KS + 8) * 2, st, a, KS);
     LAUNCH_CHECK();
+    if (a.splits > 1) {
+        hipLaunchKernelGGL(w4_join_kernel, dim3((unsigned)(((long long)a.rows * a.N + 255) / 256)), dim3(256), 0, st, a);
+        LAUNCH_CHECK();
+    }
     return VLT5_OK;
 }
-// The shares of a reduction: as many as leave no more than one workgroup per CU (256), since what a workgroup stages is then read once per CU;
-// never more than there are chunks.  Measured: 3 x 14336 x 4096 in 1 / 2 / 4 / 8 shares 15.7 / 11.6 / 11.3 / 13.9 us (rule: 2), 5 x 4097 x 14336
-// 39.6 / 25.7 / 16.6 / 21.6 (rule: 4; with 8 the 257th workgroup runs alone), 80 x 2304 x 768 5.3 / 4.8 / 5.2 / 5.7 (2), 1 x 768 x 768
-// 4.9 / 4.2 / 3.8 / 3.5 (8), 16 x 32200 x 768 6.0 / 7.1 / 9.3 / 13.3 (1).
+// How a reduction is shared.  Waves of a workgroup: as many as leave no more than one workgroup per CU (256), since what a workgroup stages is
+// then read once per CU; never more than there are chunks.  Measured: 3 x 14336 x 4096 in 1 / 2 / 4 / 8 shares 15.7 / 11.6 / 11.3 / 13.9 us (rule:
+// 2), 5 x 4097 x 14336 39.6 / 25.7 / 16.6 / 21.6 (rule: 4; with 8 the 257th workgroup runs alone), 80 x 2304 x 768 5.3 / 4.8 / 5.2 / 5.7 (2),
+// 1 x 768 x 768 4.9 / 4.2 / 3.8 / 3.5 (8), 16 x 32200 x 768 6.0 / 7.1 / 9.3 / 13.3 (1).
+// Workgroups: where the rows of x are long (VLT5_W4_SPLIT_BYTES and more for a row tile) and CUs idle, runs of about 64 KB of them go to workgroups
+// of their own, for the price of a second launch (21 x 137 x 11552: 17.4 -> 8.8 us, 16 x 500 x 8192 12.4 -> 8.1, 5 x 500 x 14336 10.0 -> 8.3; runs of 32
+// or 96 KB: 9.1 / 9.0, 8.5 / 8.7, 7.6 / 9.0).
+struct W4Plan { int kw, splits; };
+W4Plan w4_plan(int rows, int N, int K) {
+    const long long tiles = (N + 15) / 16, blocks = (rows + 15) / 16;
+    const int chunks = (K + 127) / 128;
+    W4Plan p = {8, 1};
+    while (p.kw > 1 && ((tiles * p.kw + 7) / 8 * blocks > 256 || p.kw / 2 >= chunks)) p.kw /= 2;
+    const long long wgs = (tiles * p.kw + 7) / 8 * blocks, bytes = 2LL * (rows < 16 ? rows : 16) * K;
+    if (bytes >= VLT5_W4_SPLIT_BYTES && wgs <= 128) {
+        const long long idle = 256 / wgs, runs = (bytes + 65535) / 65536;
+        p.splits = (int)(idle < runs ? idle : runs);
+    }
+    return p;
+}
 template <int G>
-int w4_shares(const W4Args& a, hipStream_t st) {
-    const long long tiles = (a.N + 15) / 16, blocks = (a.rows + 15) / 16;
-    const int chunks = (a.K + 127) / 128;
-    int kw = 8;
-    while (kw > 1 && ((tiles * kw + 7) / 8 * blocks > 256 || kw / 2 >= chunks)) kw /= 2;
+int w4_shares(const W4Args& a, int kw, hipStream_t st) {
     if (kw == 8) return w4_launch<G, 8>(a, st);
     if (kw == 4) return w4_launch<G, 4>(a, st);
     if (kw == 2) return w4_launch<G, 2>(a, st);
@@ -278,20 +308,30 @@ extern "C" int vlt5_quant_w4(const float* w_f32, const void* w_bf16, long long l
     return VLT5_OK;
 }
 
+extern "C" long long vlt5_decode_linear_w4_workspace_bytes(int rows, int N, int K) {
+    if (rows <= 0 || rows > VLT5_W4_MAX_ROWS || N <= 0 || N > 1 << 28 || K <= 0 || K > 1 << 28) return -1;
+    const int sp = w4_plan(rows, N, K).splits;
+    return sp == 1 ? 0 : 4LL * sp * rows * N;
+}
+
 extern "C" int vlt5_decode_linear_w4(const vlt5_decode_linear_w4_desc* d, void* stream) {
     if (!d || !d->x_bf16 || !d->codes || !d->scales || (!d->out_bf16 && !d->out_f32)) return VLT5_ERR_ARG;
     if (d->rows <= 0 || d->rows > VLT5_W4_MAX_ROWS || d->N <= 0 || d->N > 1 << 28 || d->K <= 0 || d->K > 1 << 28 || d->ldx < d->K) return VLT5_ERR_ARG;
     if (d->group != 32 && d->group != 64 && d->group != 128) return VLT5_ERR_ARG;
     if ((d->out_bf16 && d->ld_out_bf16 < d->N) || (d->out_f32 && d->ld_out_f32 < d->N) || (d->resid && d->ld_resid < d->N)) return VLT5_ERR_ARG;
-    if ((d->K & 31) || (d->ldx & 7) || (((uintptr_t)d->x_bf16 | (uintptr_t)d->codes) & 15)) return VLT5_ERR_ALIGN;
+    if ((d->K & 31) || (d->ldx & 7) || (((uintptr_t)d->x_bf16 | (uintptr_t)d->codes | (uintptr_t)d->workspace) & 15)) return VLT5_ERR_ALIGN;
     W4Args a;
     a.x = (const bf16_t*)d->x_bf16; a.ldx = d->ldx; a.codes = (const unsigned char*)d->codes; a.scales = (const bf16_t*)d->scales;
     a.rows = d->rows; a.N = d->N; a.K = d->K; a.groups = (d->K + d->group - 1) / d->group;
     a.alpha = d->alpha == 0.f ? 1.f : d->alpha;
     a.out_b = (bf16_t*)d->out_bf16; a.ldo = d->ld_out_bf16; a.out_f = d->out_f32; a.ldf = d->ld_out_f32;
     a.resid = d->resid; a.ldr = d->ld_resid; a.relu = d->relu;
+    const W4Plan plan = w4_plan(a.rows, a.N, a.K);
+    a.splits = plan.splits;
+    a.part = (float*)d->workspace;
+    if (plan.splits > 1 && (!d->workspace || d->workspace_bytes < vlt5_decode_linear_w4_workspace_bytes(a.rows, a.N, a.K))) return VLT5_ERR_ARG;
     hipStream_t st = (hipStream_t)stream;
-    if (d->group == 32) return w4_shares<32>(a, st);
-    if (d->group == 64) return w4_shares<64>(a, st);
-    return w4_shares<128>(a, st);
+    if (d->group == 32) return w4_shares<32>(a, plan.kw, st);
+    if (d->group == 64) return w4_shares<64>(a, plan.kw, st);
+    return w4_shares<128>(a, plan.kw, st);
 }

@@ -456,7 +456,12 @@ def decode_linear_w4(x, w, *, alpha=1.0, resid=None, relu=False, out_f32=False, 
     if rows:
         o = out.data_ptr()
         d = L.DecodeLinearW4Desc(x.data_ptr(), _row_stride(x, rows, K), codes.data_ptr(), scales.data_ptr(), rows, N, K, group, alpha, None if f32 else o, ldo,
-                                 o if f32 else None, ldo, rp, ldr, relu)
+                                 o if f32 else None, ldo, rp, ldr, relu, None, 0)
+        if 2 * min(rows, 16) * K >= L.W4_SPLIT_BYTES:                                # (below, the reduction stays within a workgroup)
+            need = lib().vlt5_decode_linear_w4_workspace_bytes(rows, N, K)
+            if need > 0:
+                ws = torch.empty(need, device=dev, dtype=torch.uint8)
+                d.workspace, d.workspace_bytes = ws.data_ptr(), need
         check(lib().vlt5_decode_linear_w4(C.byref(d), st), "vlt5_decode_linear_w4")
     return out
 
