@@ -355,6 +355,19 @@ def test_chunks(dev, ops, kind, d, hk, g, page, new, lens):
         check_attn(ops, dev, c, table, new, lens, hk * g, causal=causal, seed=g)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("d,g,new,nd", [(64, 1, 20, 0), (64, 3, 13, 40), (64, 1, 63, 0), (128, 1, 17, 0), (128, 4, 10, 16), (128, 2, 32, 0)])
+def test_few_rows_on_a_full_chip(dev, ops, kind, d, g, new, nd):
+    """Enough sequences that two row tiles share the keys they read: 17 to 64 rows, ragged, with empty sequences and one whose keys end inside a step."""
+    B, hk = 66, 8
+    lens = [170 - (7 * b) % 90 for b in range(B)]
+    news = [max(0, min(n, new - (b % 5) * (new // 6))) for b, n in enumerate(lens)]
+    news[3] = lens[4] = news[4] = 0
+    c, table = make_cache(ops, dev, lens, hk, d, 16, kind, seed=new + d)
+    bias = 2 * torch.randn(hk * g, nd, generator=gen(nd)) if nd else None
+    check_attn(ops, dev, c, table, news, lens, hk * g, scale=1.0 if nd else None, bias=bias, seed=1)
+
+
 @pytest.mark.parametrize("new,lens,nd", [([1, 1, 1], [1, 40, 300], 32), ([1, 1], [2000, 129], 128), ([20, 150], [20, 400], 128), ([65], [1000], 1), ([3], [70], 500)])
 @pytest.mark.parametrize("kind", KINDS)
 def test_relative_bias(dev, ops, kind, new, lens, nd):

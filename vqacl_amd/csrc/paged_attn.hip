@@ -93,10 +93,10 @@ struct KeyStep {
     }
 };
 
-// NW waves share the keys of a row tile in steps of 32, the next step's rows on their way while one is used; the page ids of a wave's next 32
-// steps come with one load, two to a step.
-template <int T, int DK, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void paged_attn_kernel(const PagedAttnArgs a) {
+// NW waves share the keys of 16 R rows in steps of 32, the next step's rows on their way while one is used; the page ids of a wave's next 32 steps
+// come with one load, two to a step.  The R row tiles use the same operands of K and V: a key is read and converted once for all of them.
+template <int T, int DK, int NW, int R>
+__global__ __launch_bounds__(NW * 64, R * DK > 128 ? 1 : 2) void paged_attn_kernel(const PagedAttnArgs a) {
     constexpr int NF = DK / 32, ND = DK / 16;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, kq = lane >> 4;
     int id = blockIdx.x;
@@ -104,39 +104,51 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_kernel(const PagedAttnA
     const int rt = id % a.row_tiles; id /= a.row_tiles;
     const int hk = id % a.Hkv, b = id / a.Hkv;
     const PagedSeq sq = paged_seq(a.s, b);
-    const int rows = min(sq.nq, a.s.max_q) * a.g;
-    if (rt * 16 >= rows) return;
-    const int r = min(rt * 16 + r16, rows - 1);
-    const int tok = r / a.g, hq = hk * a.g + r % a.g;
-    const int p0 = sq.len - sq.nq, pos = p0 + tok;                                 // this row's position (negative: more new tokens than keys)
-    const int L = a.causal ? min(pos + 1, sq.len) : sq.len;                       // keys this row sees
-    const int first = p0 + rt * 16 / a.g, last = p0 + min(rt * 16 + 15, rows - 1) / a.g;
+    const int rows = min(sq.nq, a.s.max_q) * a.g, r0 = rt * 16 * R;
+    if (r0 >= rows) return;
+    const int p0 = sq.len - sq.nq;
+    int pos[R], L[R], head[R];                                                     // position of this lane's row (negative: more new tokens than keys), keys it sees, its head
+    bf16x8_t fq[R][NF];                                                            // d in the order of the keys' 16-byte pieces
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int r = min(r0 + i * 16 + r16, rows - 1), tok = r / a.g;
+        head[i] = r % a.g;
+        pos[i] = p0 + tok;
+        L[i] = a.causal ? min(pos[i] + 1, sq.len) : sq.len;
+        const bf16_t* qrow = a.q + (size_t)(sq.q0 + tok) * a.q_st + (hk * a.g + head[i]) * DK;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) fq[i][f] = *reinterpret_cast<const bf16x8_t*>(qrow + (T == VLT5_KV_BF16 ? f * 32 + kq * 8 : (f >> 1) * 64 + kq * 16 + (f & 1) * 8));
+    }
+    const int first = p0 + r0 / a.g, last = p0 + min(r0 + 16 * R - 1, rows - 1) / a.g;
     const int Lmin = a.causal ? first + 1 : sq.len, Lmax = max(a.causal ? last + 1 : sq.len, 0);
     const int per = ((Lmax + a.splits - 1) / a.splits + 32 * NW - 1) / (32 * NW) * (32 * NW);
     const int lo = min(sp * per, Lmax), hi = min(lo + per, Lmax);
 
-    // d in the order of the keys' 16-byte pieces
-    bf16x8_t fq[NF];
-    const bf16_t* qrow = a.q + (size_t)(sq.q0 + tok) * a.q_st + hq * DK;
-#pragma unroll
-    for (int i = 0; i < NF; ++i) fq[i] = *reinterpret_cast<const bf16x8_t*>(qrow + (T == VLT5_KV_BF16 ? i * 32 + kq * 8 : (i >> 1) * 64 + kq * 16 + (i & 1) * 8));
     __shared__ float sb[BIAS_LDS];
     const bool near_lds = a.bias && a.g * a.nd <= BIAS_LDS;
     if (near_lds) {
         for (int i = threadIdx.x; i < a.g * a.nd; i += NW * 64) sb[i] = a.bias[(size_t)hk * a.g * a.nd + i];
         __syncthreads();
     }
-    const float* bias = a.bias ? a.bias + (size_t)hq * a.nd : nullptr;
-    const float* lbias = sb + (hq - hk * a.g) * a.nd;
-    float bias_far = bias ? bias[a.nd - 1] : 0.f;
-    arrived(bias_far);
+    const float* bias = a.bias ? a.bias + (size_t)hk * a.g * a.nd : nullptr;
+    float bias_far[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        bias_far[i] = bias ? bias[head[i] * a.nd + a.nd - 1] : 0.f;
+        arrived(bias_far[i]);
+    }
     // scores and their maximum are kept as q k (times the key's scale), with a bias as scale * q k + bias; `unit` makes powers of two of them
     const float unit = bias ? LOG2E : a.scale * LOG2E, lag = fminf(8.f / unit, 1e38f);
 
-    f32x4_t o[ND];
+    f32x4_t o[R][ND];
+    float m[R], l[R];
 #pragma unroll
-    for (int j = 0; j < ND; ++j) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
+    for (int i = 0; i < R; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < ND; ++j) o[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
     const int steps = hi > lo ? (hi - lo + 31) / 32 : 0, mine = steps > w ? (steps - w + NW - 1) / NW : 0;
     auto at = [&](int i) { return lo + (i * NW + w) * 32; };
     int ids = -1;                                                                  // lane j: page of the 16 keys j & 1 of step (i & ~31) + j / 2
@@ -152,13 +164,14 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_kernel(const PagedAttnA
         pg[buf][1] = __builtin_amdgcn_readlane(ids, (i & 31) * 2 + 1);
         st[buf].load(a, hk, pg[buf], at(i), r16, kq);
     };
-    auto use = [&](int i, int buf) {
+    auto use = [&](int step, int buf) {
         KeyStep<T, DK>& x = st[buf];
-        const int t0 = at(i);
-        f32x4_t sc[2];
+        const int t0 = at(step);
+        f32x4_t sc[R][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            sc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < R; ++q) sc[q][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int f = 0; f < NF; ++f) {
                 bf16x8_t fk;
@@ -167,91 +180,102 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_kernel(const PagedAttnA
                     const uint2 c0 = codes_to_bf16<T>(x.k[i][f >> 1][(f & 1) * 2]), c1 = codes_to_bf16<T>(x.k[i][f >> 1][(f & 1) * 2 + 1]);
                     fk = __builtin_bit_cast(bf16x8_t, make_uint4(c0.x, c0.y, c1.x, c1.y));
                 }
-                sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fk, fq[f], sc[i], 0, 0, 0);
+#pragma unroll
+                for (int q = 0; q < R; ++q) sc[q][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fk, fq[q][f], sc[q][i], 0, 0, 0);
             }
         }
         const bool whole = t0 + 32 <= min(Lmin, hi) && pg[buf][0] >= 0 && pg[buf][1] >= 0;
-        float p[2][4], top = -INFINITY;
+        bf16x8_t fp[R];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float kk[4] = {1.f, 1.f, 1.f, 1.f};
-            if constexpr (KvType<T>::SCALED) { kk[0] = x.ks[i].x; kk[1] = x.ks[i].y; kk[2] = x.ks[i].z; kk[3] = x.ks[i].w; }
+        for (int q = 0; q < R; ++q) {
+            float p[2][4], top = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) p[i][e] = sc[i][e] * kk[e];
-        }
-        if (bias) {
-            if (first - (t0 + 31) >= a.nd - 1) {                                   // every key further than the table reaches
+            for (int i = 0; i < 2; ++i) {
+                float kk[4] = {1.f, 1.f, 1.f, 1.f};
+                if constexpr (KvType<T>::SCALED) { kk[0] = x.ks[i].x; kk[1] = x.ks[i].y; kk[2] = x.ks[i].z; kk[3] = x.ks[i].w; }
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) p[i][e] = fmaf(p[i][e], a.scale, bias_far);
-            } else if (near_lds) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) p[i][e] = fmaf(p[i][e], a.scale, lbias[min(max(pos - (t0 + i * 16 + kq * 4 + e), 0), a.nd - 1)]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) p[i][e] = fmaf(p[i][e], a.scale, bias[min(max(pos - (t0 + i * 16 + kq * 4 + e), 0), a.nd - 1)]);
+                for (int e = 0; e < 4; ++e) p[i][e] = sc[q][i][e] * kk[e];
             }
-        }
-        if (!whole) {
-            asm volatile("");                                                      // (a branch, not selects in every step)
+            if (bias) {
+                if (first - (t0 + 31) >= a.nd - 1) {                               // every key further than the table reaches
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) p[i][e] = fmaf(p[i][e], a.scale, bias_far[q]);
+                } else if (near_lds) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            p[i][e] = fmaf(p[i][e], a.scale, sb[head[q] * a.nd + min(max(pos[q] - (t0 + i * 16 + kq * 4 + e), 0), a.nd - 1)]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            p[i][e] = fmaf(p[i][e], a.scale, bias[head[q] * a.nd + min(max(pos[q] - (t0 + i * 16 + kq * 4 + e), 0), a.nd - 1)]);
+                }
+            }
+            if (!whole) {
+                asm volatile("");                                                  // (a branch, not selects in every step)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[i][e] = pg[buf][i] >= 0 && t0 + i * 16 + kq * 4 + e < L[q] ? p[i][e] : -INFINITY;
+            }
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) p[i][e] = pg[buf][i] >= 0 && t0 + i * 16 + kq * 4 + e < L ? p[i][e] : -INFINITY;
-        }
+                for (int e = 0; e < 4; ++e) top = fmaxf(top, p[i][e]);
+            // the running maximum moves only when a new one is more than 2^8 away: until then probabilities up to 256 do no harm (f32 sums, bf16
+            // relative to the value), and neither the exchange between the row's four lanes nor the rescaling is needed
+            if (__any(top > m[q] + lag)) {
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float mn = fmaxf(m[q], top), ms = mn == -INFINITY ? 0.f : mn;    // a row that has seen no key yet stays at -inf, sum 0
+                const float fix = exp2_hw((m[q] - ms) * unit);
+                m[q] = mn;
+                l[q] *= fix;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+                for (int j = 0; j < ND; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top = fmaxf(top, p[i][e]);
-        // the running maximum moves only when a new one is more than 2^8 away: until then probabilities up to 256 do no harm (f32 sums, bf16
-        // relative to the value), and neither the exchange between the row's four lanes nor the rescaling is needed
-        if (__any(top > m + lag)) {
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float mn = fmaxf(m, top), ms = mn == -INFINITY ? 0.f : mn;        // a row that has seen no key yet stays at -inf, sum 0
-            const float fix = exp2_hw((m - ms) * unit);
-            m = mn;
-            l *= fix;
-#pragma unroll
-            for (int j = 0; j < ND; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[j][e] *= fix;
-        }
-        const float ms = m == -INFINITY ? 0.f : m;
-        uint32_t pb[2][2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float vv[4] = {1.f, 1.f, 1.f, 1.f}, y[4];
-            if constexpr (KvType<T>::SCALED) { vv[0] = x.vs[i].x; vv[1] = x.vs[i].y; vv[2] = x.vs[i].z; vv[3] = x.vs[i].w; }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float pe = exp2_hw((p[i][e] - ms) * unit);
-                l += pe;
-                y[e] = pe * vv[e];
+                    for (int e = 0; e < 4; ++e) o[q][j][e] *= fix;
             }
-            if (!whole) {                                                          // what lies behind the last key may hold anything, NaN too
+            const float ms = m[q] == -INFINITY ? 0.f : m[q];
+            uint32_t pb[2][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float vv[4] = {1.f, 1.f, 1.f, 1.f}, y[4];
+                if constexpr (KvType<T>::SCALED) { vv[0] = x.vs[i].x; vv[1] = x.vs[i].y; vv[2] = x.vs[i].z; vv[3] = x.vs[i].w; }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int t = t0 + i * 16 + kq * 4 + e;
-                    const bool in = pg[buf][i] >= 0 && t < sq.len;
-                    if (!(in && t < L)) y[e] = 0.f;
-                    if (!in) x.v[i][e] = VRow<T, DK>{};
+                    const float pe = exp2_hw((p[i][e] - ms) * unit);
+                    l[q] += pe;
+                    y[e] = pe * vv[e];
                 }
+                if (!whole) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = pg[buf][i] >= 0 && t0 + i * 16 + kq * 4 + e < L[q] ? y[e] : 0.f;
+                }
+                pb[i][0] = pack_bf16x2(y[0], y[1]);
+                pb[i][1] = pack_bf16x2(y[2], y[3]);
             }
-            pb[i][0] = pack_bf16x2(y[0], y[1]);
-            pb[i][1] = pack_bf16x2(y[2], y[3]);
+            fp[q] = __builtin_bit_cast(bf16x8_t, make_uint4(pb[0][0], pb[0][1], pb[1][0], pb[1][1]));
         }
-        const bf16x8_t fp = __builtin_bit_cast(bf16x8_t, make_uint4(pb[0][0], pb[0][1], pb[1][0], pb[1][1]));
+        if (!whole) {                                                              // what lies behind the last key may hold anything, NaN too
+            asm volatile("");
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (!(pg[buf][i] >= 0 && t0 + i * 16 + kq * 4 + e < sq.len)) x.v[i][e] = VRow<T, DK>{};
+        }
 #pragma unroll
         for (int j = 0; j < ND; ++j) {
             const uint4 fv = make_uint4(vpair<T, DK>(x.v[0][0], x.v[0][1], j), vpair<T, DK>(x.v[0][2], x.v[0][3], j), vpair<T, DK>(x.v[1][0], x.v[1][1], j),
                                         vpair<T, DK>(x.v[1][2], x.v[1][3], j));
-            o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, fv), fp, o[j], 0, 0, 0);
+#pragma unroll
+            for (int q = 0; q < R; ++q) o[q][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, fv), fp[q], o[q][j], 0, 0, 0);
         }
     };
     if (mine) {
@@ -259,7 +283,9 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_kernel(const PagedAttnA
         load(0, 0);
     }
 #pragma unroll
-    for (int i = 0; i < NF; ++i) arrived(fq[i]);
+    for (int q = 0; q < R; ++q)
+#pragma unroll
+        for (int f = 0; f < NF; ++f) arrived(fq[q][f]);
     int i = 0;
     for (; i + 2 < mine; i += 2) {                                                 // (every load unconditional, or the waits could not be counted)
         load(i + 1, 1);                                                            // (i is even: never the first of 32 steps)
@@ -275,45 +301,48 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_kernel(const PagedAttnA
     } else if (i < mine) {
         use(i, 0);
     }
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    m = bias ? m : m * a.scale;
 
-    // ---- the waves' shares of the keys meet in LDS, always in the order of the waves ----
+    // ---- the waves' shares of the keys meet in LDS, always in the order of the waves, one row tile after the other ----
     __shared__ float so[NW][16][DK + 4];
     __shared__ float sm[NW][16], sl[NW][16];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int q = 0; q < R; ++q) {
+        l[q] += __shfl_xor(l[q], 16, 64);
+        l[q] += __shfl_xor(l[q], 32, 64);
+        if (q) __syncthreads();
 #pragma unroll
-        for (int j = 0; j < ND; ++j) so[w][r16][(kq * 4 + e) * ND + j] = o[j][e];      // row of the A operand (kq * 4 + e) stands for d = that * ND + j
-    if (lane < 16) { sm[w][lane] = m; sl[w][lane] = l; }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 16 * (DK / 4); i += NW * 64) {
-        const int rr = i / (DK / 4), d = i % (DK / 4) * 4;
-        if (rt * 16 + rr >= rows) continue;
-        float mx = sm[0][rr];
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int ww = 1; ww < NW; ++ww) mx = fmaxf(mx, sm[ww][rr]);
-        const float ms = mx == -INFINITY ? 0.f : mx;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float sum = 0.f;
+            for (int j = 0; j < ND; ++j) so[w][r16][(kq * 4 + e) * ND + j] = o[q][j][e];      // row of the A operand (kq * 4 + e) stands for d = that * ND + j
+        if (lane < 16) { sm[w][lane] = bias ? m[q] : m[q] * a.scale; sl[w][lane] = l[q]; }
+        __syncthreads();
+        for (int k = threadIdx.x; k < 16 * (DK / 4); k += NW * 64) {
+            const int rr = k / (DK / 4), d = k % (DK / 4) * 4, r = r0 + q * 16 + rr;
+            if (r >= rows) continue;
+            float mx = sm[0][rr];
 #pragma unroll
-        for (int ww = 0; ww < NW; ++ww) {
-            const float f = exp2_hw((sm[ww][rr] - ms) * LOG2E);
-            const float4 x = *reinterpret_cast<const float4*>(&so[ww][rr][d]);
-            sum += sl[ww][rr] * f;
-            acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
-        }
-        const int tk = (rt * 16 + rr) / a.g, hh = hk * a.g + (rt * 16 + rr) % a.g;
-        const size_t token = (size_t)(sq.q0 + tk);
-        if (a.splits == 1) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            *reinterpret_cast<uint2*>(a.out + token * a.o_st + hh * DK + d) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-            if (a.lse && d == 0) a.lse[token * a.H + hh] = sum == 0.f ? -INFINITY : mx + logf(sum);
-        } else {
-            const size_t at = ((size_t)sp * a.s.n_tok + token) * a.H + hh;
-            *reinterpret_cast<float4*>(a.part_o + at * DK + d) = acc;
-            if (d == 0) { a.part_ml[at * 2] = mx; a.part_ml[at * 2 + 1] = sum; }
+            for (int ww = 1; ww < NW; ++ww) mx = fmaxf(mx, sm[ww][rr]);
+            const float ms = mx == -INFINITY ? 0.f : mx;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float sum = 0.f;
+#pragma unroll
+            for (int ww = 0; ww < NW; ++ww) {
+                const float f = exp2_hw((sm[ww][rr] - ms) * LOG2E);
+                const float4 x = *reinterpret_cast<const float4*>(&so[ww][rr][d]);
+                sum += sl[ww][rr] * f;
+                acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
+            }
+            const int hh = hk * a.g + r % a.g;
+            const size_t token = (size_t)(sq.q0 + r / a.g);
+            if (a.splits == 1) {
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                *reinterpret_cast<uint2*>(a.out + token * a.o_st + hh * DK + d) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+                if (a.lse && d == 0) a.lse[token * a.H + hh] = sum == 0.f ? -INFINITY : mx + logf(sum);
+            } else {
+                const size_t row = ((size_t)sp * a.s.n_tok + token) * a.H + hh;
+                *reinterpret_cast<float4*>(a.part_o + row * DK + d) = acc;
+                if (d == 0) { a.part_ml[row * 2] = mx; a.part_ml[row * 2 + 1] = sum; }
+            }
         }
     }
 }
@@ -695,6 +724,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
     if (a.lse && lane == 0) a.lse[row] = sum == 0.f ? -INFINITY : mx + logf(sum);
 }
 
+template <int T, int DK>
+void rows_launch(const PagedAttnArgs& a, unsigned blocks, int waves, int tiles, hipStream_t st) {
+    if (waves == 1) hipLaunchKernelGGL((paged_attn_kernel<T, DK, 1, 1>), dim3(blocks), dim3(64), 0, st, a);
+    else if (tiles == 1) hipLaunchKernelGGL((paged_attn_kernel<T, DK, 4, 1>), dim3(blocks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((paged_attn_kernel<T, DK, 4, 2>), dim3(blocks), dim3(256), 0, st, a);
+}
 template <int T, int DK, bool BIAS, int KS>
 int chunk_launch(const PagedAttnArgs& a, unsigned blocks, hipStream_t st) {
     static std::atomic<unsigned long long> done{0};
@@ -705,29 +740,42 @@ int chunk_launch(const PagedAttnArgs& a, unsigned blocks, hipStream_t st) {
     return VLT5_OK;
 }
 
-// The plan of a call, from what the host knows.  Up to 64 rows (tokens x heads of a group) go through the first kernel, more share their keys
-// through LDS.  A row tile's keys are shared by one wave up to 128 of them, else by four (80 sequences x 58 keys, 12 heads: 6.0 against 8.0 us;
-// 100 x 500: 20.4 against 19.1), and by as many workgroups as give every CU two, none with less than 512 keys (1 x 131071 keys, 8 kv heads of 128,
-// int8: 67 us in 64 shares; 8 x 2000 keys: 15 us in 3 shares of 667, 17 in 7 of 286).  Large tiles that leave a CU one workgroup get twice the
-// waves, half the keys each (8 sequences of 200 tokens over 712 keys, 12 heads: 28.4 -> 20.5 us; where CUs have two anyway it costs 5 %).
 // query heads a multiple of the kv heads; rows are counted in 32 bits
 bool paged_heads_ok(const vlt5_paged_attn_desc* d) {
     return d->H > 0 && d->H <= 1024 && d->H % d->kv.n_kv_heads == 0 && (long long)d->seqs.n_tok * d->H <= 0x7fffffffLL - 4096;
 }
-struct PagedPlan { int chunk, row_tiles, splits, waves; };
+// The plan of a call, from what the host knows.
+//   Up to 64 rows (tokens x heads of a group) go through the first kernel, more share their keys through LDS.  Where tiles of 16 rows fill the chip
+//   (512 workgroups), 17 and more rows are better off reading every key once for two tiles (20 x 20 rows over 2000 keys 25.1 -> 20.1 us, 32 x 24 over
+//   8000 152 -> 124, 41 x 40 over 10130 198 -> 182; a chip that is not full loses: 20 x 33 over 600 9.9 -> 12.3), in a bf16 cache, which has nothing
+//   to convert, from 33 on through LDS (4 x 40 over 20000 81 -> 71, 100 x 33 over 400 36 -> 27; int8 182 -> 308).
+//   A row tile's keys are shared by one wave up to 128 of them, else by four (80 x 58 keys, 12 heads: 6.0 against 8.0 us; 100 x 500: 20.4 against
+//   19.1), and by as many workgroups as give every CU two, none with less than 512 keys (1 x 131071 keys, 8 kv heads of 128, int8: 67 us in 64
+//   shares; 8 x 2000 keys: 15 us in 3 shares of 667, 17 in 7 of 286).
+//   Large tiles that leave a CU one workgroup get twice the waves, half the keys each (8 x 200 tokens over 712 keys, 12 heads: 28.4 -> 20.5 us; where
+//   CUs have two anyway it costs 5 %), and are shared out until every CU has that one (1 x 500 over 4000 33.6 -> 29.6; two a CU: twice the sums to join).
+struct PagedPlan { int chunk, row_tiles, splits, waves, tiles; };              // tiles: of 16 rows that a wave of the first kernel takes
 PagedPlan paged_plan(const vlt5_paged_attn_desc* d, const PagedSeqs& s) {
     const int g = d->H / d->kv.n_kv_heads;
-    const long long rows = (long long)s.max_q * g;
+    const long long rows = (long long)s.max_q * g, pairs = (long long)s.B * d->kv.n_kv_heads;
     const long long most_kv = d->max_kv > 0 ? d->max_kv : (long long)d->seqs.max_pages * d->kv.page_size;
+    auto share = [&](long long n) {                                            // ... of the keys between n workgroups
+        n = n < most_kv / (VLT5_PAGED_SHARED_KV / 2) ? n : most_kv / (VLT5_PAGED_SHARED_KV / 2);
+        return (int)(n < 1 ? 1 : (n > 64 ? 64 : n));
+    };
     PagedPlan p;
-    p.chunk = rows > 64;
-    const int per = p.chunk ? 128 : 16;
-    p.row_tiles = (int)((rows + per - 1) / per);
-    const long long tiles = (long long)s.B * d->kv.n_kv_heads * p.row_tiles;
-    long long sp = (512 + tiles - 1) / tiles;
-    sp = sp < most_kv / (VLT5_PAGED_SHARED_KV / 2) ? sp : most_kv / (VLT5_PAGED_SHARED_KV / 2);
-    p.splits = (int)(sp < 1 ? 1 : (sp > 64 ? 64 : sp));
-    p.waves = p.chunk ? (tiles * p.splits <= 256 ? 8 : 4) : (most_kv <= 128 ? 1 : 4);
+    auto small = [&](int tiles) {
+        const long long n = (rows + 16 * tiles - 1) / (16 * tiles) * pairs;
+        p.chunk = 0; p.tiles = tiles; p.row_tiles = (int)(n / pairs); p.splits = share((512 + n - 1) / n); p.waves = most_kv <= 128 ? 1 : 4;
+        return n * p.splits;
+    };
+    if (rows <= 64) {
+        const bool full = small(1) >= 512;
+        if (rows <= 16 || p.waves == 1 || !full) return p;
+        if (rows <= 32 || d->kv.type != VLT5_KV_BF16) { small(2); return p; }
+    }
+    const long long n = (rows + 127) / 128 * pairs;
+    p.chunk = 1; p.tiles = 0; p.row_tiles = (int)(n / pairs); p.splits = share(256 / n); p.waves = n * p.splits <= 256 ? 8 : 4;
     return p;
 }
 
@@ -775,8 +823,7 @@ extern "C" int vlt5_paged_attn(const vlt5_paged_attn_desc* d, void* stream) {
     int lrc = VLT5_OK;
 #define PA(T, D) do { if (plan.chunk && plan.waves == 8) lrc = a.bias ? chunk_launch<T, D, true, 2>(a, (unsigned)(tiles * a.splits), st) : chunk_launch<T, D, false, 2>(a, (unsigned)(tiles * a.splits), st); \
                       else if (plan.chunk) lrc = a.bias ? chunk_launch<T, D, true, 1>(a, (unsigned)(tiles * a.splits), st) : chunk_launch<T, D, false, 1>(a, (unsigned)(tiles * a.splits), st); \
-                      else if (plan.waves == 1) hipLaunchKernelGGL((paged_attn_kernel<T, D, 1>), dim3((unsigned)(tiles * a.splits)), dim3(64), 0, st, a); \
-                      else hipLaunchKernelGGL((paged_attn_kernel<T, D, 4>), dim3((unsigned)(tiles * a.splits)), dim3(256), 0, st, a); } while (0)
+                      else rows_launch<T, D>(a, (unsigned)(tiles * a.splits), plan.waves, plan.tiles, st); } while (0)
     if (c.d_kv == 64) {
         if (c.type == VLT5_KV_BF16) PA(VLT5_KV_BF16, 64); else if (c.type == VLT5_KV_INT8) PA(VLT5_KV_INT8, 64); else PA(VLT5_KV_FP8, 64);
     } else {
