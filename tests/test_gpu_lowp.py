@@ -700,3 +700,17 @@ def test_a_cold_call_inside_a_capture_and_two_graphs(dev, ops):
         assert torch.equal(ops.paged_attn(qs[2], c, t, n, scale=0.09), want[2])
         torch.cuda.synchronize()
         assert torch.equal(graphs[i][1], want[i])
+
+
+def test_no_factor_and_no_sequences(dev, ops):
+    from vqacl_amd._lib import Vlt5Error
+    w = ops.quant_w4(torch.randn(8, 64, generator=gen(1)).to(dev), 32)
+    with pytest.raises(Vlt5Error):
+        ops.decode_linear_w4(torch.zeros(1, 64, device=dev, dtype=torch.bfloat16), w, alpha=0.0)
+    none = torch.zeros(0, 3, device=dev, dtype=torch.int32)
+    c = ops.kv_pages(2, 1, 64, 16, torch.int8, dev)
+    k, v = ops.kv_page_read(c, none, none[:, 0].contiguous(), 5)
+    assert k.shape == v.shape == (0, 5, 64)
+    x = torch.zeros(0, 64, device=dev, dtype=torch.bfloat16)
+    ops.kv_page_write(c, x, x, none, none[:, 0].contiguous())
+    assert ops.paged_attn(x, c, none, none[:, 0].contiguous()).shape == (0, 64)

@@ -120,6 +120,13 @@ def test_attention_refusals(built):
     assert L.vlt5_paged_attn(C.byref(desc(seq={"n_tok": 0})), None) == 0
 
 
+def test_a_bias_table_past_32_bits_is_refused(built):
+    f = built.lib().vlt5_paged_attn
+    for n_dist in (1 << 29, (1 << 29) + 1, 0x7fffffff):
+        d = built.PagedAttnDesc(kv=built.PagedKV(**KV), seqs=built.PagedSeqs(**SEQ), q=P, q_st=256, out=P, o_st=256, H=4, scale=1.0, causal=1, rel_bias=P, n_dist=n_dist)
+        assert f(C.byref(d), None) == ARG
+
+
 def test_wrappers_refuse_host_tensors(built):
     from vqacl_amd import ops
     c = ops.KVPages(*(torch.zeros(2, 1, 16, 64, dtype=torch.int8) for _ in range(2)), *(torch.zeros(2, 1, 16) for _ in range(2)))

@@ -795,7 +795,7 @@ extern "C" int vlt5_paged_attn(const vlt5_paged_attn_desc* d, void* stream) {
     const vlt5_paged_kv& c = d->kv;
     if (!paged_heads_ok(d)) return VLT5_ERR_ARG;
     if (d->q_st < (long long)d->H * c.d_kv || d->o_st < (long long)d->H * c.d_kv) return VLT5_ERR_ARG;
-    if (d->rel_bias && (d->n_dist <= 0 || !d->causal)) return VLT5_ERR_ARG;
+    if (d->rel_bias && (d->n_dist <= 0 || !d->causal || (long long)d->H * d->n_dist > 0x7fffffffLL)) return VLT5_ERR_ARG;      // (indexed in 32 bits)
     if (!(d->scale > 0.f && d->scale <= 3.402823466e38f)) return VLT5_ERR_ARG;
     if ((d->q_st & 7) || (d->o_st & 7) || (((uintptr_t)d->q | (uintptr_t)d->out | (uintptr_t)d->workspace) & 15)) return VLT5_ERR_ALIGN;
     if (d->seqs.n_tok == 0) return VLT5_OK;

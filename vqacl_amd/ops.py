@@ -426,13 +426,15 @@ def quant_w4(w, group=128):
 
 
 def decode_linear_w4(x, w, *, alpha=1.0, resid=None, relu=False, out_f32=False, out=None):
-    """act(alpha * x W^T (+ resid)) for a few rows x bf16 [rows <= 256, K] against a `W4Weight`; resid f32 [rows, N].  Returns bf16, or f32
-    with out_f32; `out` takes the result instead (its type decides; it may be `resid` itself)."""
+    """act(alpha * x W^T (+ resid)) for a few rows x bf16 [rows <= 256, K] against a `W4Weight`; resid f32 [rows, N]; alpha not 0.  Returns
+    bf16, or f32 with out_f32; `out` takes the result instead (its type decides; it may be `resid` itself)."""
     codes, scales, group = w
     dev = x.device
     at, st = _here(x)
     if group not in (32, 64, 128):
         raise L.Vlt5Error(f"group: 32, 64 or 128, got {group}")
+    if not alpha:                                                                    # (which the library takes for 1)
+        raise L.Vlt5Error("alpha: 0 is not a factor")
     if x.dim() != 2 or codes.dim() != 2:
         _refuse(dev, ("x", x, (BF16,), (None, None), False), ("codes", codes, (torch.uint8,), (None, None), True))
     (rows, K), (N, K2) = x.shape, codes.shape
@@ -516,7 +518,8 @@ def kv_page_write(cache, k, v, table, kv_lens, *, cu_q=None, max_q=None):
     """New keys | values k, v bf16 [tokens, kv heads * d_kv] (any token stride) into the pages of their sequences, quantised on the way.
 
     table i32 [B, pages of a sequence], kv_lens i32 [B]: keys of every sequence with the new tokens counted; cu_q i32 [B + 1]: first new
-    token of every sequence (None: one token each); max_q: the most new tokens any of them has.  A page id outside the cache = not there."""
+    token of every sequence (None: one token each); max_q: the most new tokens any of them has (None: as if one had them all, which costs
+    workgroups that find nothing to do).  A page id outside the cache = not there."""
     dev = k.device
     at, st = _here(k)
     if k.dim() != 2:
@@ -536,7 +539,7 @@ def kv_page_read(cache, table, kv_lens, T):
     kv, seqs, h, d, B = _paged(cache, table, kv_lens, None, 0, None, at, dev)
     k = torch.empty(B, T, h * d, device=dev, dtype=BF16)
     v = torch.empty(B, T, h * d, device=dev, dtype=BF16)
-    if T:
+    if T and B:
         check(lib().vlt5_kv_page_read(C.byref(kv), C.byref(seqs), T, k.data_ptr(), v.data_ptr(), st), "vlt5_kv_page_read")
     return k, v
 
