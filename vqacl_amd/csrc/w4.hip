@@ -266,11 +266,12 @@ int w4_launch(const W4Args& a, hipStream_t st) {
 // then read once per CU; never more than there are chunks.  Measured: 3 x 14336 x 4096 in 1 / 2 / 4 / 8 shares 15.7 / 11.6 / 11.3 / 13.9 us (rule:
 // 2), 5 x 4097 x 14336 39.6 / 25.7 / 16.6 / 21.6 (rule: 4; with 8 the 257th workgroup runs alone), 80 x 2304 x 768 5.3 / 4.8 / 5.2 / 5.7 (2),
 // 1 x 768 x 768 4.9 / 4.2 / 3.8 / 3.5 (8), 16 x 32200 x 768 6.0 / 7.1 / 9.3 / 13.3 (1).
-// Workgroups: where a row tile of x is long (VLT5_W4_SPLIT_BYTES and more) and CUs idle, or so long (160 KB) that reading it is what a workgroup spends
-// its time on, the reduction is split for the price of a second launch: as many waves on columns as let the chip (256 workgroups; two a CU where their
-// rows fit twice) take runs of 96 KB and less, and no run much below 64 KB.  21 x 137 x 11552: 17.4 -> 8.8 us (runs of 32 or 96 KB: 9.1 / 9.0),
-// 16 x 500 x 8192 12.4 -> 8.1, 5 x 500 x 14336 10.0 -> 8.3; 16 x 4096 x 14336 in 1 / 2 / 4 / 8 runs 23.0 / 18.0 / 14.9 / 14.6, 64 x 4097 x 8192 in 1 / 2 / 4
-// 31.5 / 34.7 / 26.1; below 160 KB a full chip gains nothing: 16 x 4096 x 4096 7.7 -> 9.4, 5 x 4097 x 14336 16.1 -> 16.1.
+// Workgroups: where a row tile of x is so long that reading it is what a workgroup spends its time on (VLT5_W4_SPLIT_BYTES where half the CUs idle,
+// 140 KB where nearly so, 160 KB on a full chip), the reduction is split for the price of a second launch: as many waves on columns as let 256
+// workgroups (two a CU where nothing else will do) take runs of 96 KB and less, and no run much below 64 KB.  21 x 137 x 11552: 17.4 -> 8.8 us (runs
+// of 32 or 96 KB: 9.1 / 9.0), 16 x 500 x 8192 12.4 -> 8.1, 5 x 4097 x 14336 16.2 -> 14.6; 16 x 4096 x 14336 in 1 / 2 / 4 / 8 runs 23.0 / 18.0 / 14.9 /
+// 14.6, 64 x 4097 x 8192 in 1 / 2 / 4 31.5 / 34.7 / 26.1.  Shorter rows gain nothing: 8 x 4112 x 8192 11.8 -> 13.1 (129 workgroups, 128 KB), 8 x 4096 x
+// 8192 10.4 -> 10.5, 5 x 8000 x 14336 17.7 -> 17.8 (full chip, 128 and 140 KB).
 struct W4Plan { int kw, splits; };
 W4Plan w4_plan(int rows, int N, int K) {
     const long long tiles = (N + 15) / 16, blocks = (rows + 15) / 16;
@@ -279,12 +280,11 @@ W4Plan w4_plan(int rows, int N, int K) {
     while (p.kw > 1 && ((tiles * p.kw + 7) / 8 * blocks > 256 || p.kw / 2 >= chunks)) p.kw /= 2;
     auto wgs = [&](int kw) { return (tiles * kw + 7) / 8 * blocks; };
     const long long bytes = 2LL * (rows < 16 ? rows : 16) * K, runs = (bytes + 65535) / 65536;
-    if (bytes >= VLT5_W4_SPLIT_BYTES && (wgs(p.kw) <= 128 || bytes >= 160 * 1024))
+    if (bytes >= (wgs(p.kw) <= 128 ? VLT5_W4_SPLIT_BYTES : wgs(p.kw) <= 136 ? 140 * 1024 : 160 * 1024))
         for (int kw = p.kw; kw; kw /= 2) {
             const long long w = wgs(kw);
             long long sp = 256 / w;
-            if ((256 + w / 8) / w > sp && bytes <= (sp + 1) * 72 * 1024) ++sp;
-            if (sp > runs || (kw == 1 && w * runs <= 512 + w / 8)) sp = runs;
+            if (sp > runs || (kw == 1 && bytes > sp * 96 * 1024 && w * runs <= 544)) sp = runs;
             if (sp > 1 && (kw == 1 || bytes <= sp * 96 * 1024)) {
                 p.kw = kw; p.splits = (int)sp;
                 break;
