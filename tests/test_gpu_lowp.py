@@ -589,6 +589,31 @@ def test_decode_linear_w4_slabs_with_a_short_end(dev, ops):
         assert bool(((z - want).abs() <= acc + U * want + H * want).all())
 
 
+@pytest.mark.parametrize("rows,N,K,group", [(256, 1100, 7712, 64), (250, 2100, 4128, 32), (129, 2053, 8224, 128), (241, 9001, 992, 128), (255, 8452, 1024, 32)])
+def test_decode_linear_w4_many_rows(dev, ops, rows, N, K, group):
+    """More than 2^31 multiply-adds: 32 rows a workgroup, split and not, ends inside a chunk and inside a group, rows and columns past the last tile."""
+    from vqacl_amd._lib import lib
+    assert rows * N * K > 2 ** 31 and (lib().vlt5_decode_linear_w4_workspace_bytes(rows, N, K) > 0) == (K >= 4096)
+    g = gen(rows + N)
+    w = ops.quant_w4((torch.randn(N, K, generator=g) * K ** -0.5).to(dev), group)
+    wide = torch.full((rows, K + 8), float("nan")).to(BF)
+    x = wide[:, :K]
+    x.copy_(torch.randn(rows, K, generator=g))
+    x[2] = 0
+    v, xd = w4_value(w), wide.to(dev)[:, :K]
+    ref = x.double() @ v.t()
+    acc = (group + -(-K // group) + 16) * U * (x.double().abs() @ v.abs().t())
+    y = ops.decode_linear_w4(xd, w, out_f32=True).cpu().double()
+    assert bool(((y - ref).abs() <= acc).all()) and bool((y[2] == 0).all())
+    resid = torch.randn(rows, N, generator=g)
+    room = torch.full((rows + 2, N + 3), 7.0, device=dev, dtype=BF)
+    ops.decode_linear_w4(xd, w, alpha=-2.0, relu=True, resid=resid.to(dev), out=room[1:-1, :N])
+    want = (-2 * ref + resid.double()).clamp_min(0)
+    assert bool(((room[1:-1, :N].cpu().double() - want).abs() <= 2 * acc + U * want + H * want).all())
+    room[1:-1, :N] = 7
+    assert bool((room == 7).all())
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_more_new_tokens_than_keys(dev, ops, kind):
     """Positions below zero: nothing is written for them, they see nothing; the others are as ever."""

@@ -235,6 +235,130 @@ __global__ __launch_bounds__(512) void w4_kernel(const W4Args a, int KS) {
     }
 }
 
+// ---- product, many rows ----------------------------------------------------------------------------------------------------------
+// Above 2^31 multiply-adds the kernel above is bound by its vector instructions: each code is converted and each sum scaled for sixteen rows, and long
+// rows of x leave a CU one workgroup.  Here a workgroup has 32 rows and 128 columns, a wave 32 columns of them, on 32 x 32 x 16 instructions; chunks of
+// 128 k of x go through two buffers of LDS (row stride 272 bytes: sixteen rows of an operand start in sixteen groups of four banks), the next two on
+// their way while one is multiplied, codes and scales four chunks ahead, codes turned round through LDS as above.  The 16 k of an instruction lie in
+// one group, half of them in each half of the wave.  256 x 4096 x 14336: 100 -> 58 us (0.52 PFLOP/s), 128 x 14336 x 4096 60 -> 31, 200 x 2000 x 8192
+// 30 -> 23; what bounds it still is the vector unit (100 instructions a wave and chunk for 8 of the matrix unit).  64 rows a workgroup: 50, 33, 24.
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
+
+template <int G>
+__global__ __launch_bounds__(256, 2) void w4_many_kernel(const W4Args a) {
+    constexpr int GPC = 128 / G, DW = G / 16, KROW = 272, U = 4;               // groups of a chunk, dwords of a lane per group, chunks requested ahead
+    __shared__ __attribute__((aligned(16))) char xs[2][32 * KROW];
+    __shared__ __attribute__((aligned(16))) char turns[4][2048];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r32 = lane & 31, h = lane >> 5;
+    const int m_tile = blockIdx.y * 32, n0 = blockIdx.x * 128 + w * 32, n = n0 + r32;
+    char* turn = turns[w];
+    // loads as above: lane l has piece (l & 3), swapped within the column, of columns l >> 2 and 16 + (l >> 2); columns past the end repeat the last one
+    const int lseg = (lane & 3) ^ ((lane >> 4) & 3);
+    const unsigned char* wrow[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) wrow[j] = a.codes + (size_t)min(n0 + j * 16 + (lane >> 2), a.N - 1) * (a.K / 2);
+    const bf16_t* srow = a.scales + (size_t)min(n, a.N - 1) * a.groups;
+    const bf16_t* xrow[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) xrow[i] = a.x + (size_t)min(m_tile + i * 16 + (tid >> 4), a.rows - 1) * a.ldx;
+    const int xk = (tid & 15) * 8;
+    const int all = (a.K + 127) / 128, c0 = (int)((long long)all * blockIdx.z / a.splits), c1 = (int)((long long)all * (blockIdx.z + 1) / a.splits);
+    uint4 xr[2][2];
+    vlt5_u32x4_t cw[U][2];
+    struct Scales { bf16_t v[2 * GPC]; } sn;
+    // (past the end the last chunk again: every load unconditional, or the waits could not be counted; past the end of a row any codes, x is zero there)
+    auto fetch_x = [&](int u, int c) {
+        const int k = min(c, c1 - 1) * 128 + xk;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) xr[u][i] = *reinterpret_cast<const uint4*>(xrow[i] + (k < a.K ? k : 0));
+    };
+    auto fetch_w = [&](int u, int past) {
+        const int c = min(past, c1 - 1), at = c * 128 + lseg * 32 < a.K ? c * 64 + lseg * 16 : 0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) cw[u][j] = *reinterpret_cast<const vlt5_u32x4_t*>(wrow[j] + at);
+    };
+    auto fetch_s = [&](int c) {                                                // of chunks c + 2 h and c + 2 h + 1
+        const int at = (c + 2 * h) * GPC;
+        if (at + 2 * GPC <= a.groups) {
+            __builtin_memcpy(&sn, srow + at, sizeof sn);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2 * GPC; ++i) sn.v[i] = srow[min(at + i, a.groups - 1)];
+        }
+    };
+    auto stage = [&](int u, int c) {
+        const bool past = c * 128 + xk >= a.K;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<uint4*>(xs[u] + (i * 16 + (tid >> 4)) * KROW + xk * 2) = past ? make_uint4(0, 0, 0, 0) : xr[u][i];
+    };
+    f32x16_t tot;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) tot[e] = 0.f;
+    fetch_x(0, c0);
+    fetch_x(1, c0 + 1);
+    fetch_s(c0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) fetch_w(u, c0 + u);
+    stage(0, c0);
+    fetch_x(0, c0 + 2);
+    __syncthreads();
+    for (int c = c0; c < c1; c += U) {
+        const Scales sc = sn;
+        fetch_s(c + U);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (c + u >= c1) break;
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int j = 0; j < 2; ++j) *reinterpret_cast<vlt5_u32x4_t*>(turn + j * 1024 + lane * 16) = cw[u][j];
+            __builtin_amdgcn_wave_barrier();
+            fetch_w(u, c + u + U);
+            uint32_t sp[(GPC + 1) / 2];                                        // this chunk's scales, from the half that has them
+            if constexpr (GPC == 1) {
+                uint32_t both;
+                __builtin_memcpy(&both, &sc, 4);
+                both = __builtin_amdgcn_ds_bpermute(((u >> 1) * 32 + r32) * 4, both);
+                sp[0] = u & 1 ? both >> 16 : both;
+            } else {
+                __builtin_memcpy(sp, &sc.v[(u & 1) * GPC], sizeof sp);
+#pragma unroll
+                for (int i = 0; i < GPC / 2; ++i) sp[i] = __builtin_amdgcn_ds_bpermute(((u >> 1) * 32 + r32) * 4, sp[i]);
+            }
+#pragma unroll
+            for (int gi = 0; gi < GPC; ++gi) {
+                uint32_t cg[DW];                                               // this lane's codes of the group: 4 * DW bytes at gi * G / 2 + h * G / 4 of the column's 64
+#pragma unroll
+                for (int q = 0; q < (DW + 3) / 4; ++q) {
+                    const int byte = gi * (G / 2) + h * (G / 4) + q * 16;
+                    const char* p = turn + r32 * 64 + (((byte >> 4) ^ ((r32 >> 2) & 3)) << 4) + (byte & 15);
+                    constexpr int some = DW < 4 ? 4 * DW : 16;
+                    __builtin_memcpy(cg + q * 4, __builtin_assume_aligned(p, some), some);
+                }
+                f32x16_t acc;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+#pragma unroll
+                for (int e = 0; e < DW; ++e)
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(xs[u & 1] + r32 * KROW + (gi * G + h * (G / 2) + e * 8) * 2), fp4x8(cg[e]), acc,
+                                                                  0, 0, 0);
+                const float s = __uint_as_float(gi & 1 ? sp[gi / 2] & 0xffff0000u : sp[gi / 2] << 16);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) tot[e] = fmaf(s, acc[e], tot[e]);
+            }
+            if (c + u + 1 < c1) stage((u + 1) & 1, c + u + 1);
+            fetch_x((u + 1) & 1, c + u + 3);
+            __syncthreads();
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const int m = m_tile + e / 4 * 8 + h * 4 + e % 4;
+        if (a.splits == 1) w4_store(a, m, n, tot[e]);
+        else if (m < a.rows && n < a.N) a.part[((size_t)blockIdx.z * a.rows + m) * a.N + n] = tot[e];
+    }
+}
+
 // the runs of a split reduction, added in their order
 __global__ __launch_bounds__(256) void w4_join_kernel(const W4Args a) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x, all = (long long)a.rows * a.N;
@@ -245,6 +369,13 @@ __global__ __launch_bounds__(256) void w4_join_kernel(const W4Args a) {
     w4_store(a, (int)(i / a.N), (int)(i % a.N), s);
 }
 
+int w4_join(const W4Args& a, hipStream_t st) {
+    if (a.splits > 1) {
+        hipLaunchKernelGGL(w4_join_kernel, dim3((unsigned)(((long long)a.rows * a.N + 255) / 256)), dim3(256), 0, st, a);
+        LAUNCH_CHECK();
+    }
+    return VLT5_OK;
+}
 template <int G, int KW>
 int w4_launch(const W4Args& a, hipStream_t st) {
     static std::atomic<unsigned long long> done{0};
@@ -256,11 +387,7 @@ int w4_launch(const W4Args& a, hipStream_t st) {
     const dim3 grid(((a.N + 15) / 16 + 8 / KW - 1) / (8 / KW), (a.rows + 15) / 16, a.splits);
     hipLaunchKernelGGL((w4_kernel<G, KW>), grid, dim3(512), 8 * 1024 + rows * (KS + 8) * 2, st, a, KS);
     LAUNCH_CHECK();
-    if (a.splits > 1) {
-        hipLaunchKernelGGL(w4_join_kernel, dim3((unsigned)(((long long)a.rows * a.N + 255) / 256)), dim3(256), 0, st, a);
-        LAUNCH_CHECK();
-    }
-    return VLT5_OK;
+    return w4_join(a, st);
 }
 // How a reduction is shared.  Waves of a workgroup: as many as leave no more than one workgroup per CU (256), since what a workgroup stages is
 // then read once per CU; never more than there are chunks.  Measured: 3 x 14336 x 4096 in 1 / 2 / 4 / 8 shares 15.7 / 11.6 / 11.3 / 13.9 us (rule:
@@ -272,11 +399,21 @@ int w4_launch(const W4Args& a, hipStream_t st) {
 // of 32 or 96 KB: 9.1 / 9.0), 16 x 500 x 8192 12.4 -> 8.1, 5 x 4097 x 14336 16.2 -> 14.6; 16 x 4096 x 14336 in 1 / 2 / 4 / 8 runs 23.0 / 18.0 / 14.9 /
 // 14.6, 64 x 4097 x 8192 in 1 / 2 / 4 31.5 / 34.7 / 26.1.  Shorter rows gain nothing: 8 x 4112 x 8192 11.8 -> 13.1 (129 workgroups, 128 KB), 8 x 4096 x
 // 8192 10.4 -> 10.5, 5 x 8000 x 14336 17.7 -> 17.8 (full chip, 128 and 140 KB).
+// More than 16 rows and 2^31 multiply-adds: the other kernel (kw 0), the reduction shared by up to 512 workgroups in runs of 1024 k and more; a chip with
+// 192 workgroups shares only what is 8192 long (160 x 4096 x 4096 in 1 / 2 / 3 runs 23.3 / 22.3 / 21.6 us, 256 x 4096 x 14336 in 1 / 2 / 3 70 / 56 / 65,
+// 64 x 14336 x 4096 in 1 / 2 24.9 / 28.2).  Below, it loses: 33 x 4096 x 4096 13.0 against 11.1, 256 x 2048 x 2304 14.4 / 10.4, 128 x 4096 x 4096 17.6 / 15.2.
 struct W4Plan { int kw, splits; };
 W4Plan w4_plan(int rows, int N, int K) {
     const long long tiles = (N + 15) / 16, blocks = (rows + 15) / 16;
     const int chunks = (K + 127) / 128;
     W4Plan p = {8, 1};
+    if (rows > 16 && (double)rows * N * K > 2147483648.0) {
+        const long long w = (N + 127LL) / 128 * ((rows + 31) / 32), most = 32LL * K < VLT5_W4_SPLIT_BYTES || (w >= 192 && chunks < 64) ? 1 : chunks / 8, share = 512 / w;
+        p.kw = 0;
+        p.splits = (int)(share < most ? share : most);
+        if (p.splits < 1) p.splits = 1;
+        return p;
+    }
     while (p.kw > 1 && ((tiles * p.kw + 7) / 8 * blocks > 256 || p.kw / 2 >= chunks)) p.kw /= 2;
     auto wgs = [&](int kw) { return (tiles * kw + 7) / 8 * blocks; };
     const long long bytes = 2LL * (rows < 16 ? rows : 16) * K, runs = (bytes + 65535) / 65536;
@@ -294,6 +431,11 @@ W4Plan w4_plan(int rows, int N, int K) {
 }
 template <int G>
 int w4_shares(const W4Args& a, int kw, hipStream_t st) {
+    if (kw == 0) {
+        hipLaunchKernelGGL(w4_many_kernel<G>, dim3((a.N + 127) / 128, (a.rows + 31) / 32, a.splits), dim3(256), 0, st, a);
+        LAUNCH_CHECK();
+        return w4_join(a, st);
+    }
     if (kw == 8) return w4_launch<G, 8>(a, st);
     if (kw == 4) return w4_launch<G, 4>(a, st);
     if (kw == 2) return w4_launch<G, 2>(a, st);
