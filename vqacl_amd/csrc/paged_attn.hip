@@ -107,6 +107,24 @@ __global__ __launch_bounds__(NW * 64, R * DK > 128 ? 1 : 2) void paged_attn_kern
     const int rows = min(sq.nq, a.s.max_q) * a.g, r0 = rt * 16 * R;
     if (r0 >= rows) return;
     const int p0 = sq.len - sq.nq;
+    const int first = p0 + r0 / a.g, last = p0 + min(r0 + 16 * R - 1, rows - 1) / a.g;
+    const int Lmin = a.causal ? first + 1 : sq.len, Lmax = max(a.causal ? last + 1 : sq.len, 0);
+    const int per = ((Lmax + a.splits - 1) / a.splits + 32 * NW - 1) / (32 * NW) * (32 * NW);
+    const int lo = min(sp * per, Lmax), hi = min(lo + per, Lmax);
+
+    // what the first step needs is requested in the order it is waited for: page ids, query rows, bias, (keys and values below)
+    const int steps = hi > lo ? (hi - lo + 31) / 32 : 0, mine = steps > w ? (steps - w + NW - 1) / NW : 0;
+    auto at = [&](int i) { return lo + (i * NW + w) * 32; };
+    int ids = -1;                                                                  // lane j: page of the 16 keys j & 1 of step (i & ~31) + j / 2
+    auto load_ids = [&](int i) {
+        const int t = at(i + (lane >> 1)) + (lane & 1) * 16;
+        ids = i + (lane >> 1) < mine && t < hi ? a.s.table[(size_t)b * a.s.max_pages + (t >> a.s.page_shift)] : -1;
+    };
+    auto settle_ids = [&] {
+        arrived(ids);
+        if ((unsigned)ids >= (unsigned)a.s.n_pages) ids = -1;
+    };
+    if (mine) load_ids(0);
     int pos[R], L[R], head[R];                                                     // position of this lane's row (negative: more new tokens than keys), keys it sees, its head
     bf16x8_t fq[R][NF];                                                            // d in the order of the keys' 16-byte pieces
 #pragma unroll
@@ -119,24 +137,17 @@ __global__ __launch_bounds__(NW * 64, R * DK > 128 ? 1 : 2) void paged_attn_kern
 #pragma unroll
         for (int f = 0; f < NF; ++f) fq[i][f] = *reinterpret_cast<const bf16x8_t*>(qrow + (T == VLT5_KV_BF16 ? f * 32 + kq * 8 : (f >> 1) * 64 + kq * 16 + (f & 1) * 8));
     }
-    const int first = p0 + r0 / a.g, last = p0 + min(r0 + 16 * R - 1, rows - 1) / a.g;
-    const int Lmin = a.causal ? first + 1 : sq.len, Lmax = max(a.causal ? last + 1 : sq.len, 0);
-    const int per = ((Lmax + a.splits - 1) / a.splits + 32 * NW - 1) / (32 * NW) * (32 * NW);
-    const int lo = min(sp * per, Lmax), hi = min(lo + per, Lmax);
-
     __shared__ float sb[BIAS_LDS];
     const bool near_lds = a.bias && a.g * a.nd <= BIAS_LDS;
-    if (near_lds) {
-        for (int i = threadIdx.x; i < a.g * a.nd; i += NW * 64) sb[i] = a.bias[(size_t)hk * a.g * a.nd + i];
-        __syncthreads();
-    }
     const float* bias = a.bias ? a.bias + (size_t)hk * a.g * a.nd : nullptr;
+    float table[2];
+    if (near_lds)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) table[i] = bias[min((int)threadIdx.x + i * NW * 64, a.g * a.nd - 1)];
     float bias_far[R];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        bias_far[i] = bias ? bias[head[i] * a.nd + a.nd - 1] : 0.f;
-        arrived(bias_far[i]);
-    }
+    for (int i = 0; i < R; ++i) bias_far[i] = bias ? bias[head[i] * a.nd + a.nd - 1] : 0.f;
+    if (mine) settle_ids();
     // scores and their maximum are kept as q k (times the key's scale), with a bias as scale * q k + bias; `unit` makes powers of two of them
     const float unit = bias ? LOG2E : a.scale * LOG2E, lag = fminf(8.f / unit, 1e38f);
 
@@ -149,14 +160,6 @@ __global__ __launch_bounds__(NW * 64, R * DK > 128 ? 1 : 2) void paged_attn_kern
 #pragma unroll
         for (int j = 0; j < ND; ++j) o[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
-    const int steps = hi > lo ? (hi - lo + 31) / 32 : 0, mine = steps > w ? (steps - w + NW - 1) / NW : 0;
-    auto at = [&](int i) { return lo + (i * NW + w) * 32; };
-    int ids = -1;                                                                  // lane j: page of the 16 keys j & 1 of step (i & ~31) + j / 2
-    auto load_ids = [&](int i) {
-        const int t = at(i + (lane >> 1)) + (lane & 1) * 16;
-        ids = i + (lane >> 1) < mine && t < hi ? paged_page(a.s, b, t) : -1;
-        arrived(ids);
-    };
     int pg[2][2];
     KeyStep<T, DK> st[2];
     auto load = [&](int i, int buf) {
@@ -278,19 +281,28 @@ __global__ __launch_bounds__(NW * 64, R * DK > 128 ? 1 : 2) void paged_attn_kern
             for (int q = 0; q < R; ++q) o[q][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, fv), fp[q], o[q][j], 0, 0, 0);
         }
     };
-    if (mine) {
-        load_ids(0);
-        load(0, 0);
-    }
+    if (mine) load(0, 0);
 #pragma unroll
-    for (int q = 0; q < R; ++q)
+    for (int q = 0; q < R; ++q) {
 #pragma unroll
         for (int f = 0; f < NF; ++f) arrived(fq[q][f]);
+        arrived(bias_far[q]);
+    }
+    if (near_lds) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if ((int)threadIdx.x + k * NW * 64 < a.g * a.nd) sb[threadIdx.x + k * NW * 64] = table[k];
+        for (int k = threadIdx.x + 2 * NW * 64; k < a.g * a.nd; k += NW * 64) sb[k] = bias[k];
+        __syncthreads();
+    }
     int i = 0;
     for (; i + 2 < mine; i += 2) {                                                 // (every load unconditional, or the waits could not be counted)
         load(i + 1, 1);                                                            // (i is even: never the first of 32 steps)
         use(i, 0);
-        if (((i + 2) & 31) == 0) load_ids(i + 2);
+        if (((i + 2) & 31) == 0) {
+            load_ids(i + 2);
+            settle_ids();
+        }
         load(i + 2, 0);
         use(i + 1, 1);
     }
@@ -347,6 +359,11 @@ __global__ __launch_bounds__(NW * 64, R * DK > 128 ? 1 : 2) void paged_attn_kern
     }
 }
 
+// Room for the chunk kernel's bias tables, one per head of the group: distances from -PAD on (keys past a row's own, masked) to PAD past the last
+// entry, so that a tile's 32 entries of a lane lie at fixed places from one address (8 x 100 - 200 tokens over 712 keys, 12 heads of 64, int8, 128
+// distances: 20.5 -> XX us; 45 x 79 over 79 13.2 -> YY; without a bias 18.0 and 9.5).
+constexpr int CHUNK_BIAS_LDS = 2048, PAD = 96;
+
 // ---- chunks: many rows share the keys ------------------------------------------------------------------------------------------------
 // 128 query rows a workgroup, 32 of them a wave; tiles of 64 keys and values are converted to bf16 ONCE per workgroup on their way into LDS
 // (two buffers: the next tile's loads are in flight while one is used), the same two products as above on 32 x 32 x 16 instructions.
@@ -358,7 +375,7 @@ __global__ __launch_bounds__(NW * 64, R * DK > 128 ? 1 : 2) void paged_attn_kern
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 
 template <int T, int DK, bool BIAS, int KS>
-__global__ __launch_bounds__(256 * KS, 2) void paged_chunk_kernel(const PagedAttnArgs a) {
+__global__ __launch_bounds__(256 * KS, DK == 64 && KS == 1 ? 3 : 2) void paged_chunk_kernel(const PagedAttnArgs a) {
     constexpr int NT = DK / 32, NKS = DK / 16, BY = KvType<T>::BYTES, ROWB = DK * BY;
     constexpr int KROW = DK * 2 + 16, KBYTES = 64 * KROW, VBYTES = 4 * NT * 1024, BUF = KBYTES + VBYTES + 512;
     constexpr int KCH = ROWB / 16, KP = 64 * KCH / 256;                                 // 16-byte pieces of a key row; pieces of a thread
@@ -376,27 +393,47 @@ __global__ __launch_bounds__(256 * KS, 2) void paged_chunk_kernel(const PagedAtt
     const int wr0 = rt * 128 + w4 * 32;                                                 // first row of the wave
     const int r = min(wr0 + r32, rows - 1);
     const int tok = r / a.g, hq = hk * a.g + r % a.g;
-    const int pos = sq.len - sq.nq + tok;
-    const int L = a.causal ? min(pos + 1, sq.len) : sq.len;
     const int p0 = sq.len - sq.nq;
+    const int L = a.causal ? p0 + tok + 1 : sq.len;                                     // keys of this lane's row (with a bias its position is L - 1)
     const int Lmax = max(a.causal ? p0 + min(rt * 128 + 127, rows - 1) / a.g + 1 : sq.len, 0);
     const int wLmin = a.causal ? p0 + min(wr0, rows - 1) / a.g + 1 : sq.len;            // the wave's rows all see the keys below this ...
     const int wLmax = wr0 < rows ? (a.causal ? p0 + min(wr0 + 31, rows - 1) / a.g + 1 : sq.len) : 0;      // ... and none those from here on
     const int per = ((Lmax + a.splits - 1) / a.splits + 63) & ~63;
     const int lo = min(sp * per, Lmax), hi = min(lo + per, Lmax);
 
+    // what the first tile needs is requested in the order it is waited for: page ids, query rows, bias, (keys and values below)
+    // the keys of 16 are in one page; lane j: page of the j-th 16 keys of the 16 tiles from (tile & ~15) on, or -1
+    int ids = -1, pg[4], pn[4];                                                         // ... and those of this tile and the next
+    const int tiles = (hi - lo + 63) / 64;
+    auto load_ids = [&](int tile) {
+        const int t = lo + tile * 64 + lane * 16;
+        ids = t < hi ? a.s.table[(size_t)b * a.s.max_pages + (t >> a.s.page_shift)] : -1;
+    };
+    auto settle_ids = [&] {
+        arrived(ids);
+        if ((unsigned)ids >= (unsigned)a.s.n_pages) ids = -1;
+    };
+    if (half < tiles) load_ids(0);
     bf16x8_t fq[NKS];
     const bf16_t* qrow = a.q + (size_t)(sq.q0 + tok) * a.q_st + hq * DK;
 #pragma unroll
     for (int i = 0; i < NKS; ++i) fq[i] = *reinterpret_cast<const bf16x8_t*>(qrow + i * 16 + h * 8);
     const float* bias = BIAS ? a.bias + (size_t)hq * a.nd : nullptr;
     float bias_far = BIAS ? bias[a.nd - 1] : 0.f;
-    arrived(bias_far);
     float* sb = reinterpret_cast<float*>(smem + 2 * KS * BUF);
-    const bool near_lds = BIAS && a.g * a.nd <= BIAS_LDS;
-    const float* lbias = sb + (hq - hk * a.g) * a.nd;
+    const int span = min(a.nd, CHUNK_BIAS_LDS) + 2 * PAD, entries = a.g * span;          // (larger tables do not fit)
+    const bool near_lds = BIAS && entries <= CHUNK_BIAS_LDS;
+    const float* lbias = sb + (hq - hk * a.g) * span + PAD - 59;                        // (59: the largest key of a lane in a tile, not counting 4 h)
+    auto entry = [&](int i) {
+        int hh = 0;
+        for (; i >= span; i -= span) ++hh;
+        return a.bias[((size_t)hk * a.g + hh) * a.nd + min(max(i - PAD, 0), a.nd - 1)];
+    };
+    float table[2];
     if (near_lds)
-        for (int i = tid; i < a.g * a.nd; i += 256 * KS) sb[i] = a.bias[(size_t)hk * a.g * a.nd + i];      // (the barrier before the first tile covers it)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) table[j] = entry(min(tid + j * 256 * KS, entries - 1));
+    settle_ids();
     // scores and their maximum are kept as q k (times the key's scale), with a bias as scale * q k + bias; `unit` makes powers of two of them
     const float unit = BIAS ? LOG2E : a.scale * LOG2E, lag = fminf(8.f / unit, 1e38f);
 
@@ -405,14 +442,6 @@ __global__ __launch_bounds__(256 * KS, 2) void paged_chunk_kernel(const PagedAtt
     uint32_t vr[8][VW];
     float ksc = 0.f, vsc = 0.f;
     bool sees = false;
-    // the keys of 16 are in one page; lane j: page of the j-th 16 keys of the 16 tiles from (tile & ~15) on, or -1
-    int ids = -1, pg[4], pn[4];                                                         // ... and those of this tile and the next
-    const int tiles = (hi - lo + 63) / 64;
-    auto load_ids = [&](int tile) {
-        const int t = lo + tile * 64 + lane * 16;
-        ids = t < hi ? paged_page(a.s, b, t) : -1;
-        arrived(ids);
-    };
     auto first_row = [&](int page, int t) { return (((size_t)max(page, 0) * a.Hkv + hk) << a.s.page_shift) + (t & ((1 << a.s.page_shift) - 1)); };
     auto fetch = [&](int tile) {
         const int t0 = lo + tile * 64;
@@ -493,13 +522,17 @@ __global__ __launch_bounds__(256 * KS, 2) void paged_chunk_kernel(const PagedAtt
         for (int e = 0; e < 16; ++e) o[j][e] = 0.f;
     float m = -INFINITY, l = 0.f;
     char* mine = smem + half * 2 * BUF;
-    if (half < tiles) {
-        load_ids(0);
-        fetch(half);
-        stage(mine);
-    }
+    if (half < tiles) fetch(half);
 #pragma unroll
     for (int i = 0; i < NKS; ++i) arrived(fq[i]);
+    arrived(bias_far);
+    if (near_lds) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            if (tid + j * 256 * KS < entries) sb[tid + j * 256 * KS] = table[j];
+        for (int i = tid + 512 * KS; i < entries; i += 256 * KS) sb[i] = entry(i);
+    }
+    if (half < tiles) stage(mine);
     __syncthreads();
     for (int turn = 0; turn * KS < tiles; ++turn) {
         const int tile = turn * KS + half, t0 = lo + tile * 64, cur = turn & 1;
@@ -508,7 +541,10 @@ __global__ __launch_bounds__(256 * KS, 2) void paged_chunk_kernel(const PagedAtt
 #pragma unroll
         for (int i = 0; i < 4; ++i) pg[i] = pn[i];
         if (more) {
-            if (((tile + KS) & 15) == half) load_ids((tile + KS) & ~15);
+            if (((tile + KS) & 15) == half) {
+                load_ids((tile + KS) & ~15);
+                settle_ids();
+            }
             fetch(tile + KS);
         }
         if (t0 < wLmax && tile < tiles) {
@@ -540,11 +576,13 @@ __global__ __launch_bounds__(256 * KS, 2) void paged_chunk_kernel(const PagedAtt
 #pragma unroll
                         for (int e = 0; e < 16; ++e) s[i][e] = fmaf(s[i][e], a.scale, bias_far);
                 } else if (near_lds) {
+                    // a row's distances here: at least -94 (its wave's last row sees the tile's first key), at most nd + 92 (the first row's nearest is in the table)
+                    const float* lb = lbias + (L - 1 - t0 - h * 4);
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            s[i][e] = fmaf(s[i][e], a.scale, lbias[min(max(pos - (t0 + i * 32 + e / 4 * 8 + h * 4 + e % 4), 0), a.nd - 1)]);
+                            s[i][e] = fmaf(s[i][e], a.scale, lb[59 - (i * 32 + e / 4 * 8 + e % 4)]);
                             if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);          // (all 32 in flight would not leave registers for the sums)
                         }
                 } else {
@@ -552,7 +590,7 @@ __global__ __launch_bounds__(256 * KS, 2) void paged_chunk_kernel(const PagedAtt
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            s[i][e] = fmaf(s[i][e], a.scale, bias[min(max(pos - (t0 + i * 32 + e / 4 * 8 + h * 4 + e % 4), 0), a.nd - 1)]);
+                            s[i][e] = fmaf(s[i][e], a.scale, bias[min(max(L - 1 - (t0 + i * 32 + e / 4 * 8 + h * 4 + e % 4), 0), a.nd - 1)]);
                             if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                         }
                 }
@@ -733,7 +771,7 @@ void rows_launch(const PagedAttnArgs& a, unsigned blocks, int waves, int tiles, 
 template <int T, int DK, bool BIAS, int KS>
 int chunk_launch(const PagedAttnArgs& a, unsigned blocks, hipStream_t st) {
     static std::atomic<unsigned long long> done{0};
-    constexpr int bytes = 2 * KS * (64 * (DK * 2 + 16) + 4 * (DK / 32) * 1024 + 512) + (BIAS ? BIAS_LDS * 4 : 0);
+    constexpr int bytes = 2 * KS * (64 * (DK * 2 + 16) + 4 * (DK / 32) * 1024 + 512) + (BIAS ? CHUNK_BIAS_LDS * 4 : 0);
     const int rc = vlt5_lds_optin((const void*)paged_chunk_kernel<T, DK, BIAS, KS>, bytes, done);
     if (rc) return rc;
     hipLaunchKernelGGL((paged_chunk_kernel<T, DK, BIAS, KS>), dim3(blocks), dim3(256 * KS), bytes, st, a);
