@@ -791,20 +791,23 @@ bool paged_heads_ok(const vlt5_paged_attn_desc* d) {
 //   19.1), and by as many workgroups as give every CU two, none with less than 512 keys (1 x 131071 keys, 8 kv heads of 128, int8: 67 us in 64
 //   shares; 8 x 2000 keys: 15 us in 3 shares of 667, 17 in 7 of 286).
 //   Large tiles that leave a CU one workgroup get twice the waves, half the keys each (8 x 200 tokens over 712 keys, 12 heads: 28.4 -> 20.5 us; where
-//   CUs have two anyway it costs 5 %), and are shared out until every CU has that one (1 x 500 over 4000 33.6 -> 29.6; two a CU: twice the sums to join).
+//   CUs have two anyway it costs 5 %), and are shared out until every CU has that one (1 x 500 over 4000 33.6 -> 29.6; two a CU: twice the sums to
+//   join), none with less than 341 keys (1 x 40 over 2000, 32 query and 4 kv heads of 128: 24.1 us with 512 and more, 20.2 with 341, 18.7 with 256;
+//   2 x 128 over 3000, 8 heads: 25.0, 21.8, 25.9).
 struct PagedPlan { int chunk, row_tiles, splits, waves, tiles; };              // tiles: of 16 rows that a wave of the first kernel takes
 PagedPlan paged_plan(const vlt5_paged_attn_desc* d, const PagedSeqs& s) {
     const int g = d->H / d->kv.n_kv_heads;
     const long long rows = (long long)s.max_q * g, pairs = (long long)s.B * d->kv.n_kv_heads;
     const long long most_kv = d->max_kv > 0 ? d->max_kv : (long long)d->seqs.max_pages * d->kv.page_size;
-    auto share = [&](long long n) {                                            // ... of the keys between n workgroups
-        n = n < most_kv / (VLT5_PAGED_SHARED_KV / 2) ? n : most_kv / (VLT5_PAGED_SHARED_KV / 2);
+    auto share = [&](long long n, int parts) {                                 // ... of the keys between n workgroups, at least 1024 / parts for one
+        const long long most = most_kv < VLT5_PAGED_SHARED_KV ? 1 : most_kv / (VLT5_PAGED_SHARED_KV / parts);
+        n = n < most ? n : most;
         return (int)(n < 1 ? 1 : (n > 64 ? 64 : n));
     };
     PagedPlan p;
     auto small = [&](int tiles) {
         const long long n = (rows + 16 * tiles - 1) / (16 * tiles) * pairs;
-        p.chunk = 0; p.tiles = tiles; p.row_tiles = (int)(n / pairs); p.splits = share((512 + n - 1) / n); p.waves = most_kv <= 128 ? 1 : 4;
+        p.chunk = 0; p.tiles = tiles; p.row_tiles = (int)(n / pairs); p.splits = share((512 + n - 1) / n, 2); p.waves = most_kv <= 128 ? 1 : 4;
         return n * p.splits;
     };
     if (rows <= 64) {
@@ -813,7 +816,7 @@ PagedPlan paged_plan(const vlt5_paged_attn_desc* d, const PagedSeqs& s) {
         if (rows <= 32 || d->kv.type != VLT5_KV_BF16) { small(2); return p; }
     }
     const long long n = (rows + 127) / 128 * pairs;
-    p.chunk = 1; p.tiles = 0; p.row_tiles = (int)(n / pairs); p.splits = share(256 / n); p.waves = n * p.splits <= 256 ? 8 : 4;
+    p.chunk = 1; p.tiles = 0; p.row_tiles = (int)(n / pairs); p.splits = share(256 / n, 3); p.waves = n * p.splits <= 256 ? 8 : 4;
     return p;
 }
 
