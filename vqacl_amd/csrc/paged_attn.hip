@@ -13,7 +13,7 @@
 //
 // Single tokens are bound by the bytes of the cache: 32 x 16384 keys, 8 kv heads of 128, e4m3: 148 us = 5.5 TB/s; 1 x 131071, int8: 42 us =
 // 6.6 TB/s (a part of it from the last-level cache) and 4.6 us to join its 64 shares.  Long chunks are bound by the matrix and vector units
-// together (42 % and 41 % busy at the 1.8 GHz such a load runs at): 2048 tokens over 16384 bf16 keys, 32 heads of 128: 570-590 us = 890 TFLOP/s.
+// together (42 % and 41 % busy at the 1.8 GHz such a load runs at): 2048 tokens over 16384 bf16 keys, 32 heads of 128: 545-590 us = 875-945 TFLOP/s.
 #include "paged.h"
 
 namespace {
