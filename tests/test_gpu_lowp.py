@@ -739,3 +739,15 @@ def test_no_factor_and_no_sequences(dev, ops):
     x = torch.zeros(0, 64, device=dev, dtype=torch.bfloat16)
     ops.kv_page_write(c, x, x, none, none[:, 0].contiguous())
     assert ops.paged_attn(x, c, none, none[:, 0].contiguous()).shape == (0, 64)
+
+
+@pytest.mark.parametrize("alpha", [1e-50, -1e-50, 2.0 ** -150, -0.0])
+def test_a_factor_that_is_zero_in_f32_is_refused(dev, ops, alpha):
+    """The descriptor holds alpha in f32, where 0 stands for 1."""
+    from vqacl_amd._lib import Vlt5Error
+    w = ops.quant_w4(torch.randn(8, 64, generator=gen(1)).to(dev), 32)
+    x = torch.ones(1, 64, device=dev, dtype=BF)
+    with pytest.raises(Vlt5Error):
+        ops.decode_linear_w4(x, w, alpha=alpha)
+    small = 2.0 ** -100                                                                     # an f32 number: a factor as any other
+    assert torch.equal(ops.decode_linear_w4(x, w, alpha=small, out_f32=True), small * ops.decode_linear_w4(x, w, out_f32=True))

@@ -361,6 +361,7 @@ def enc_attn_sublayer_bwd(dy, sv, want_dscores=False):
 # ---- the token-step in low precision: 4-bit weights, a paged key/value cache, the attention over it -------------------------------
 FP8, F32, I32 = torch.float8_e4m3fn, torch.float32, torch.int32
 _KV_TYPE = {BF16: 0, torch.int8: 1, FP8: 2}
+_F32_ZERO = 2.0 ** -150                # the largest number that f32 rounds to 0 (half its smallest, a tie)
 
 
 class W4Weight(NamedTuple):
@@ -426,15 +427,15 @@ def quant_w4(w, group=128):
 
 
 def decode_linear_w4(x, w, *, alpha=1.0, resid=None, relu=False, out_f32=False, out=None):
-    """act(alpha * x W^T (+ resid)) for a few rows x bf16 [rows <= 256, K] against a `W4Weight`; resid f32 [rows, N]; alpha not 0.  Returns
+    """act(alpha * x W^T (+ resid)) for a few rows x bf16 [rows <= 256, K] against a `W4Weight`; resid f32 [rows, N]; alpha not 0 in f32.  Returns
     bf16, or f32 with out_f32; `out` takes the result instead (its type decides; it may be `resid` itself)."""
     codes, scales, group = w
     dev = x.device
     at, st = _here(x)
     if group not in (32, 64, 128):
         raise L.Vlt5Error(f"group: 32, 64 or 128, got {group}")
-    if not alpha:                                                                    # (which the library takes for 1)
-        raise L.Vlt5Error("alpha: 0 is not a factor")
+    if -_F32_ZERO <= alpha <= _F32_ZERO:                                             # (0 in the descriptor, which the library takes for 1)
+        raise L.Vlt5Error(f"alpha: {alpha} is 0 in f32, and 0 is not a factor")
     if x.dim() != 2 or codes.dim() != 2:
         _refuse(dev, ("x", x, (BF16,), (None, None), False), ("codes", codes, (torch.uint8,), (None, None), True))
     (rows, K), (N, K2) = x.shape, codes.shape
