@@ -751,3 +751,18 @@ def test_a_factor_that_is_zero_in_f32_is_refused(dev, ops, alpha):
         ops.decode_linear_w4(x, w, alpha=alpha)
     small = 2.0 ** -100                                                                     # an f32 number: a factor as any other
     assert torch.equal(ops.decode_linear_w4(x, w, alpha=small, out_f32=True), small * ops.decode_linear_w4(x, w, out_f32=True))
+
+
+@pytest.mark.parametrize("rows,N,K,group,runs", [(5, 4300, 14112, 64, 3), (6, 5000, 12320, 128, 3), (62, 4600, 5088, 32, 3), (50, 5400, 6176, 64, 4), (63, 5000, 5088, 128, 3)])
+def test_decode_linear_w4_split_on_a_chip_that_is_not_full(dev, ops, rows, N, K, group, runs):
+    """Runs on both sides of two workgroups a CU, with ends inside a chunk, a group and a tile."""
+    from vqacl_amd._lib import lib
+    assert lib().vlt5_decode_linear_w4_workspace_bytes(rows, N, K) == 4 * rows * N * runs
+    g = gen(rows + K)
+    w = ops.quant_w4((torch.randn(N, K, generator=g) * K ** -0.5).to(dev), group)
+    x = torch.randn(rows, K, generator=g).to(BF)
+    v = w4_value(w)
+    ref = x.double() @ v.t()
+    acc = (group + -(-K // group) + 16) * U * (x.double().abs() @ v.abs().t())
+    y = ops.decode_linear_w4(x.to(dev), w, out_f32=True).cpu().double()
+    assert bool(((y - ref).abs() <= acc).all())

@@ -136,3 +136,18 @@ def test_wrappers_refuse_host_tensors(built):
                  lambda: ops.kv_page_read(c, t, n, 4), lambda: ops.paged_attn(x, c, t, n)):
         with pytest.raises(built.Vlt5Error):
             call()
+
+
+def test_the_plan_of_a_product_has_no_edge_beside_one_size(built):
+    """A reduction is split by what a workgroup moves: neighbours in rows, columns and k are planned alike."""
+    size = built.lib().vlt5_decode_linear_w4_workspace_bytes
+    for N in range(4097, 5121, 31):
+        for rows, K in ((5, 13504), (5, 14304), (5, 14336), (5, 15008), (6, 12288), (16, 7936), (14, 9600)):
+            assert size(rows, N, K) > 0, (rows, N, K)
+        for rows, K in ((4, 14336), (4, 16384), (3, 16384), (5, 10240), (8, 8192), (1, 14336)):
+            assert size(rows, N, K) == 0, (rows, N, K)
+    runs = lambda rows, N, K: size(rows, N, K) // (4 * rows * N)
+    for N in range(16600, 24400, 200):                                                     # four runs for what unsplit takes as long as four: up to three rounds
+        assert runs(16, N, 8192) == 4, N
+    assert [runs(16, N, 5120) for N in (19000, 21000, 22000, 23000, 27000)] == [3, 3, 0, 0, 0]
+    assert [runs(16, N, 14336) for N in (9000, 9400, 9900)] == [7, 3, 3]

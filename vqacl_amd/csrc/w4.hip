@@ -391,14 +391,21 @@ int w4_launch(const W4Args& a, hipStream_t st) {
 }
 // How a reduction is shared.  Waves of a workgroup: as many as leave no more than one workgroup per CU (256), since what a workgroup stages is
 // then read once per CU; never more than there are chunks.  Measured: 3 x 14336 x 4096 in 1 / 2 / 4 / 8 shares 15.7 / 11.6 / 11.3 / 13.9 us (rule:
-// 2), 5 x 4097 x 14336 39.6 / 25.7 / 16.6 / 21.6 (rule: 4; with 8 the 257th workgroup runs alone), 80 x 2304 x 768 5.3 / 4.8 / 5.2 / 5.7 (2),
+// 2), 5 x 4097 x 14336 43.0 / 23.7 / 16.7 / 21.9 (4; with 8 the 257th workgroup runs alone), 80 x 2304 x 768 5.3 / 4.8 / 5.2 / 5.7 (2),
 // 1 x 768 x 768 4.9 / 4.2 / 3.8 / 3.5 (8), 16 x 32200 x 768 6.0 / 7.1 / 9.3 / 13.3 (1).
-// Workgroups: where a row tile of x is so long that reading it is what a workgroup spends its time on (VLT5_W4_SPLIT_BYTES where half the CUs idle,
-// 140 KB where nearly so, 160 KB on a full chip), the reduction is split for the price of a second launch: as many waves on columns as let 256
-// workgroups (two a CU where nothing else will do) take runs of 96 KB and less, and no run much below 64 KB.  21 x 137 x 11552: 17.4 -> 8.8 us (runs
-// of 32 or 96 KB: 9.1 / 9.0), 16 x 500 x 8192 12.4 -> 8.1, 5 x 4097 x 14336 16.2 -> 14.6; 16 x 4096 x 14336 in 1 / 2 / 4 / 8 runs 23.0 / 18.0 / 14.9 /
-// 14.6, 64 x 4097 x 8192 in 1 / 2 / 4 31.5 / 34.7 / 26.1.  Shorter rows gain nothing: 8 x 4112 x 8192 11.8 -> 13.1 (129 workgroups, 128 KB), 8 x 4096 x
-// 8192 10.4 -> 10.5, 5 x 8000 x 14336 17.7 -> 17.8 (full chip, 128 and 140 KB).
+// Workgroups: where a row tile of x is so long that reading it is what a workgroup spends its time on, the reduction is split for the price of a
+// second launch: as many waves on columns as let 256 workgroups take runs of 96 KB and less, and no run much below 64 KB.
+//   When: from 160 KB on (what does not fit LDS in one slab); VLT5_W4_SPLIT_BYTES where half the CUs idle; and where three in eight idle, from three
+//   runs on if the tile and its workgroup's codes are 288 KB together.  Of some 550 sizes (1 - 64 rows, 500 - 8192 columns, 4096 - 16384 k), unsplit
+//   against split, us, full chip: 6 x 4096 x 12288 (144 KB) 13.2 / 13.4, 6 x 4096 x 14336 (168) 15.5 / 14.7, 5 x 4096 x 16384 (160) 16.4 / 15.0;
+//   half idle: 21 x 137 x 11552 17.4 / 8.8, 16 x 500 x 8192 12.4 / 8.1; 129 to 144 workgroups: 5 x 4097 x 14336 (364) 16.7 / 15.2, 5 x 4600 x 14336
+//   16.5 / 15.5, 6 x 4368 x 12288 (336) 15.4 / 13.9, 64 x 4600 x 5088 (477) 22.6 / 18.1, 12 x 4097 x 6144 (240) 12.0 / 11.7, 8 x 4112 x 8192 (256, two
+//   runs) 12.3 / 13.0, 4 x 4097 x 16384 (384, two runs) 17.0 / 17.9; 172 of them: 5 x 5500 x 14336 16.6 / 16.9.
+//   How: two runs share a CU and take twice as long as one alone, so 256 workgroups are one round and the second 256 another; unsplit is as many
+//   rounds as there are runs.  A workgroup for every run where that is fewer (two rounds where 256 workgroups have another way): 16 x 18000 x 8192
+//   in 1 / 4 runs 32.7 / 27.3 (564 workgroups: three rounds for four), 16 x 23000 x 8192 37.2 / 33.5 (720), 16 x 25000 x 8192 38.6 / 38.3 (784: four),
+//   16 x 21000 x 5120 in 1 / 3 runs 22.7 / 19.6 (495: two for three), 16 x 23000 x 5120 22.8 / 24.9 (540: three), 16 x 19000 x 12288 in 1 / 6 53.4 /
+//   40.2 (894), 16 x 9400 x 14336 in 3 / 7 26.3 / 27.7 (222 against 518).
 // More than 16 rows and 2^31 multiply-adds: the other kernel (kw 0), the reduction shared by up to 512 workgroups in runs of 1024 k and more; a chip with
 // 192 workgroups shares only what is 8192 long (160 x 4096 x 4096 in 1 / 2 / 3 runs 23.3 / 22.3 / 21.6 us, 256 x 4096 x 14336 in 1 / 2 / 3 70 / 56 / 65,
 // 64 x 14336 x 4096 in 1 / 2 24.9 / 28.2).  Below, it loses: 33 x 4096 x 4096 13.0 against 11.1, 256 x 2048 x 2304 14.4 / 10.4, 128 x 4096 x 4096 17.6 / 15.2.
@@ -416,12 +423,13 @@ W4Plan w4_plan(int rows, int N, int K) {
     }
     while (p.kw > 1 && ((tiles * p.kw + 7) / 8 * blocks > 256 || p.kw / 2 >= chunks)) p.kw /= 2;
     auto wgs = [&](int kw) { return (tiles * kw + 7) / 8 * blocks; };
-    const long long bytes = 2LL * (rows < 16 ? rows : 16) * K, runs = (bytes + 65535) / 65536;
-    if (bytes >= (wgs(p.kw) <= 128 ? VLT5_W4_SPLIT_BYTES : wgs(p.kw) <= 136 ? 140 * 1024 : 160 * 1024))
+    auto rounds = [](long long n) { return n / 512 * 2 + (n % 512 + 255) / 256; };
+    const long long bytes = 2LL * (rows < 16 ? rows : 16) * K, runs = (bytes + 65535) / 65536, codes = 64LL / p.kw * K;
+    if (bytes >= 160 * 1024 || (wgs(p.kw) <= 128 && bytes >= VLT5_W4_SPLIT_BYTES) || (wgs(p.kw) <= 160 && runs >= 3 && bytes + codes >= 288 * 1024))
         for (int kw = p.kw; kw; kw /= 2) {
             const long long w = wgs(kw);
             long long sp = 256 / w;
-            if (sp > runs || (kw == 1 && bytes > sp * 96 * 1024 && w * runs <= 544)) sp = runs;
+            if (sp > runs || (kw == 1 && w <= 256 && bytes > sp * 96 * 1024 && (sp == 1 || w * runs <= 512) && rounds(w * runs) < runs)) sp = runs;
             if (sp > 1 && (kw == 1 || bytes <= sp * 96 * 1024)) {
                 p.kw = kw; p.splits = (int)sp;
                 break;
