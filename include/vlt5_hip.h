@@ -686,7 +686,8 @@ int vlt5_decode_attn(const vlt5_attn_desc* d, void* stream);
  * nearest e2m1 number to w / scale (f32, ties to the even code); a group with an infinity or a NaN gets the scale NaN. */
 int vlt5_quant_w4(const float* w_f32, const void* w_bf16, long long ldw, int N, int K, int group, void* codes, void* scales, void* stream);
 /* out[m, n] = act(alpha * sum_k x[m, k] value(code[n, k]) scale[n, k / group] (+ resid[m, n])), the vlt5_decode_linear of such a weight:
- * rows <= VLT5_W4_MAX_ROWS, any N, x bf16 (rows 16-byte aligned), f32 sums, bf16 and / or f32 output.  `resid` may be `out_f32`.
+ * rows <= VLT5_W4_MAX_ROWS, any N, x bf16 (rows 16-byte aligned), f32 sums, bf16 and / or f32 output.  `resid` may be `out_f32`
+ * (the same rows); any other output over an input, or over the other output, is refused.
  * workspace: vlt5_decode_linear_w4_workspace_bytes (0: none needed, always so where 2 * min(rows, 16) * K < VLT5_W4_SPLIT_BYTES), 16-byte
  * aligned, one per call in flight. */
 #define VLT5_W4_MAX_ROWS 256

@@ -766,3 +766,27 @@ def test_decode_linear_w4_split_on_a_chip_that_is_not_full(dev, ops, rows, N, K,
     acc = (group + -(-K // group) + 16) * U * (x.double().abs() @ v.abs().t())
     y = ops.decode_linear_w4(x.to(dev), w, out_f32=True).cpu().double()
     assert bool(((y - ref).abs() <= acc).all())
+
+
+def test_decode_linear_w4_outputs_beside_their_inputs(dev, ops):
+    """Slices of one buffer that share no element are taken, whatever their order; those that do are refused."""
+    from vqacl_amd._lib import Vlt5Error
+    w = ops.quant_w4(torch.randn(64, 64, generator=gen(1)).to(dev), 32)
+    first = torch.randn(20, 192, generator=gen(2)).to(BF).to(dev)
+    for rows in (1, 20):
+        for a, b in ((0, 64), (64, 0), (0, 128), (128, 64), (56, 120)):
+            buf = first.clone()
+            want = ops.decode_linear_w4(buf[:rows, a:a + 64].clone(), w)
+            got = ops.decode_linear_w4(buf[:rows, a:a + 64], w, out=buf[:rows, b:b + 64])
+            assert torch.equal(got, want) and torch.equal(buf[:rows, a:a + 64], first[:rows, a:a + 64])
+        for a, b in ((0, 0), (0, 56), (64, 8)):
+            buf = first.clone()
+            with pytest.raises(Vlt5Error):
+                ops.decode_linear_w4(buf[:rows, a:a + 64], w, out=buf[:rows, b:b + 64])
+    above = first.clone()
+    assert torch.equal(ops.decode_linear_w4(above[1:3, :64], w, out=above[4:6, 64:128]), ops.decode_linear_w4(first[1:3, :64], w))
+    two = torch.randn(6, 64, generator=gen(3)).to(dev)
+    want = ops.decode_linear_w4(first[:3, :64], w, resid=two[:3].clone(), out_f32=True)
+    assert torch.equal(ops.decode_linear_w4(first[:3, :64], w, resid=two[:3], out=two[3:]), want)
+    with pytest.raises(Vlt5Error):
+        ops.decode_linear_w4(first[:3, :64], w, resid=two[:3], out=two[1:4])

@@ -151,3 +151,19 @@ def test_the_plan_of_a_product_has_no_edge_beside_one_size(built):
         assert runs(16, N, 8192) == 4, N
     assert [runs(16, N, 5120) for N in (19000, 21000, 22000, 23000, 27000)] == [3, 3, 0, 0, 0]
     assert [runs(16, N, 14336) for N in (9000, 9400, 9900)] == [7, 3, 3]
+
+
+def test_an_output_over_an_input_of_a_product_is_refused(built):
+    """Other workgroups may still read what a workgroup would write; only `resid` may be the f32 output itself."""
+    f = built.lib().vlt5_decode_linear_w4
+    M, R, N, K = 1 << 30, 256, 8704, 1024                                                  # far apart: pointers that are never followed
+    ok = dict(x_bf16=M, ldx=K, codes=2 * M, scales=3 * M, rows=R, N=N, K=K, group=32, out_bf16=4 * M, ld_out_bf16=N)
+    wide = dict(ldx=K + N, ld_out_bf16=K + N)                                              # slices of one buffer
+    f32 = dict(out_bf16=None, out_f32=4 * M, ld_out_f32=N)
+    last = (R - 1) * 2
+    for change in (dict(out_bf16=M), dict(out_bf16=M + 16), dict(out_bf16=M + last * K + 2 * K - 16), dict(out_bf16=M - last * N - 2 * N + 16), dict(wide, out_bf16=M + 2 * K - 16),
+                   dict(wide, out_bf16=M - 2 * N + 16), dict(wide, out_bf16=M + last * (K + N) + 2 * K - 16), dict(out_bf16=M + 2 * N, ld_out_bf16=N + 8),
+                   dict(out_bf16=2 * M + N * K // 2 - 16), dict(out_bf16=3 * M - last * N - 16), dict(out_f32=4 * M, ld_out_f32=N), dict(resid=4 * M, ld_resid=N),
+                   dict(f32, out_f32=M), dict(f32, resid=4 * M + 4, ld_resid=N), dict(f32, resid=4 * M, ld_resid=N + 8)):
+        d = built.DecodeLinearW4Desc(**{**ok, **change})
+        assert f(C.byref(d), None) == ARG, change

@@ -8,6 +8,7 @@
 // gfx950 turns a pair of e2m1 codes into a pair of bf16 numbers in ONE instruction (v_cvt_scalef32_pk_bf16_fp4), exactly and with the sign,
 // so the matrix instruction gets its operand with half an instruction per weight and no zero-point term has to be subtracted from the sums.
 #include "common.h"
+#include "rows.h"
 #include "vlt5_hip.h"
 
 namespace {
@@ -481,6 +482,14 @@ extern "C" int vlt5_decode_linear_w4(const vlt5_decode_linear_w4_desc* d, void* 
     if (d->group != 32 && d->group != 64 && d->group != 128) return VLT5_ERR_ARG;
     if ((d->out_bf16 && d->ld_out_bf16 < d->N) || (d->out_f32 && d->ld_out_f32 < d->N) || (d->resid && d->ld_resid < d->N)) return VLT5_ERR_ARG;
     if ((d->K & 31) || (d->ldx & 7) || (((uintptr_t)d->x_bf16 | (uintptr_t)d->codes | (uintptr_t)d->workspace) & 15)) return VLT5_ERR_ALIGN;
+    // what is written may not lie over what other workgroups still read; `resid` may be `out_f32`: its element is read by the lane that writes it
+    const RowSpan x = {d->x_bf16, d->rows, 2 * d->ldx, 2LL * d->K}, ob = {d->out_bf16, d->rows, 2 * d->ld_out_bf16, 2LL * d->N};
+    const RowSpan of = {d->out_f32, d->rows, 4 * d->ld_out_f32, 4LL * d->N}, res = {d->resid, d->rows, 4 * d->ld_resid, 4LL * d->N};
+    const RowSpan codes = {d->codes, d->N, d->K / 2, d->K / 2}, scales = {d->scales, d->N, 2LL * ((d->K + d->group - 1) / d->group), 2LL * ((d->K + d->group - 1) / d->group)};
+    const bool in_place = d->resid == d->out_f32 && (d->rows == 1 || d->ld_resid == d->ld_out_f32);
+    if (vlt5_rows_overlap(ob, of) || (!in_place && vlt5_rows_overlap(of, res)) || vlt5_rows_overlap(ob, res)) return VLT5_ERR_ARG;
+    for (const RowSpan& in : {x, codes, scales})
+        if (vlt5_rows_overlap(ob, in) || vlt5_rows_overlap(of, in)) return VLT5_ERR_ARG;
     W4Args a;
     a.x = (const bf16_t*)d->x_bf16; a.ldx = d->ldx; a.codes = (const unsigned char*)d->codes; a.scales = (const bf16_t*)d->scales;
     a.rows = d->rows; a.N = d->N; a.K = d->K; a.groups = (d->K + d->group - 1) / d->group;

@@ -428,7 +428,8 @@ def quant_w4(w, group=128):
 
 def decode_linear_w4(x, w, *, alpha=1.0, resid=None, relu=False, out_f32=False, out=None):
     """act(alpha * x W^T (+ resid)) for a few rows x bf16 [rows <= 256, K] against a `W4Weight`; resid f32 [rows, N]; alpha not 0 in f32.  Returns
-    bf16, or f32 with out_f32; `out` takes the result instead (its type decides; it may be `resid` itself)."""
+    bf16, or f32 with out_f32; `out` takes the result instead (its type decides; it may be `resid` itself, and may
+    share no memory with anything else)."""
     codes, scales, group = w
     dev = x.device
     at, st = _here(x)
