@@ -734,6 +734,7 @@ int vlt5_kv_page_write(const vlt5_paged_kv* c, const vlt5_paged_seqs* q, const v
 int vlt5_kv_page_read(const vlt5_paged_kv* c, const vlt5_paged_seqs* q, int T, void* k_out, void* v_out, void* stream);
 /* out = softmax(scale * q K^T + bias) V of the new tokens over the keys of their sequence (which are in the cache already: write first).
  * q, out bf16 [n_tok] rows of H heads of d_kv, H a multiple of n_kv_heads (query head h reads kv head h / (H / n_kv_heads)); scale > 0.
+ * `out` may be `q` (the same rows); over q in any other way, or over the cache, it is refused.
  * causal: a token sees the positions up to its own, else all kv_lens[b].  rel_bias f32 [H][n_dist] (causal only): added to the score of a
  * key that lies `dist` positions back, the last entry for every larger dist -- T5's bucketed bias of a decoder as a function of the
  * distance.  A token that sees no key gets zeros and lse -inf.  What lies behind a sequence's last key may hold anything.  A key masked by

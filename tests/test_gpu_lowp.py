@@ -790,3 +790,23 @@ def test_decode_linear_w4_outputs_beside_their_inputs(dev, ops):
     assert torch.equal(ops.decode_linear_w4(first[:3, :64], w, resid=two[:3], out=two[3:]), want)
     with pytest.raises(Vlt5Error):
         ops.decode_linear_w4(first[:3, :64], w, resid=two[:3], out=two[1:4])
+
+
+@pytest.mark.parametrize("new,lens", [([1, 1, 1], [50, 3000, 7]), ([3, 80, 20], [50, 300, 20]), ([150], [2000])])
+def test_attention_in_the_place_of_its_queries(dev, ops, new, lens):
+    """`out` beside q in one buffer and as q itself, single tokens and chunks, split and not; over q in any other way it is refused."""
+    from vqacl_amd._lib import Vlt5Error
+    c, table = make_cache(ops, dev, lens, 2, 64, 16, torch.int8, seed=37)
+    n, args, kw = sum(new), (table.to(dev), ints(dev, lens)), dict(cu_q=ints(dev, starts(new)), max_q=max(new), scale=0.1)
+    first = torch.randn(n, 768, generator=gen(6)).to(BF).to(dev)
+    want = ops.paged_attn(first[:, 128:384].contiguous(), c, *args, **kw)
+    for a, b in ((128, 384), (128, 128), (512, 0)):
+        buf = first.clone()
+        buf[:, a:a + 256] = first[:, 128:384]
+        assert torch.equal(ops.paged_attn(buf[:, a:a + 256], c, *args, out=buf[:, b:b + 256], **kw), want)
+    with pytest.raises(Vlt5Error):
+        ops.paged_attn(first[:, :256], c, *args, out=first[:, 64:320], **kw)
+    if n > 1:
+        flat = torch.zeros(n + 1, 256, device=dev, dtype=BF)
+        with pytest.raises(Vlt5Error):
+            ops.paged_attn(flat[:n], c, *args, out=flat[1:], **kw)

@@ -167,3 +167,14 @@ def test_an_output_over_an_input_of_a_product_is_refused(built):
                    dict(f32, out_f32=M), dict(f32, resid=4 * M + 4, ld_resid=N), dict(f32, resid=4 * M, ld_resid=N + 8)):
         d = built.DecodeLinearW4Desc(**{**ok, **change})
         assert f(C.byref(d), None) == ARG, change
+
+
+def test_attention_over_its_own_queries_is_refused(built):
+    """`out` may be `q`, row for row; a workgroup that writes elsewhere in q may be ahead of one that reads there."""
+    f = built.lib().vlt5_paged_attn
+    M = 1 << 20
+    kv, seq = built.PagedKV(**{**KV, "k": 2 * M, "v": 3 * M}), built.PagedSeqs(**{**SEQ, "B": 3, "n_tok": 3})
+    for change in (dict(out=M + 16), dict(out=M + 512), dict(out=M - 16), dict(out=M, o_st=264), dict(q_st=384, o_st=384, out=M + 128), dict(q_st=520, o_st=520, out=M - 16),
+                   dict(out=M + 2 * 512 + 496), dict(out=2 * M + 4 * 2 * 16 * 64 - 16), dict(out=3 * M - 2 * 512 - 16)):
+        d = built.PagedAttnDesc(**{**dict(kv=kv, seqs=seq, q=M, q_st=256, o_st=256, H=4, scale=1.0, causal=1), **change})
+        assert f(C.byref(d), None) == ARG, change

@@ -15,6 +15,7 @@
 // 6.6 TB/s (a part of it from the last-level cache) and 4.6 us to join its 64 shares.  Long chunks are bound by the matrix and vector units
 // together (42 % and 41 % busy at the 1.8 GHz such a load runs at): 2048 tokens over 16384 bf16 keys, 32 heads of 128: 545-590 us = 875-945 TFLOP/s.
 #include "paged.h"
+#include "rows.h"
 
 namespace {
 
@@ -839,6 +840,11 @@ extern "C" int vlt5_paged_attn(const vlt5_paged_attn_desc* d, void* stream) {
     if (d->rel_bias && (d->n_dist <= 0 || !d->causal || (long long)d->H * d->n_dist > 0x7fffffffLL)) return VLT5_ERR_ARG;      // (indexed in 32 bits)
     if (!(d->scale > 0.f && d->scale <= 3.402823466e38f)) return VLT5_ERR_ARG;
     if ((d->q_st & 7) || (d->o_st & 7) || (((uintptr_t)d->q | (uintptr_t)d->out | (uintptr_t)d->workspace) & 15)) return VLT5_ERR_ALIGN;
+    // `out` may take q's place: a workgroup writes the very rows and heads that only it reads; over anything else others may still read it
+    const RowSpan q = {d->q, d->seqs.n_tok, 2 * d->q_st, 2LL * d->H * c.d_kv}, out = {d->out, d->seqs.n_tok, 2 * d->o_st, q.width};
+    const long long cache = (long long)c.n_kv_heads * c.page_size * c.d_kv * (c.type == VLT5_KV_BF16 ? 2 : 1);
+    if (!(d->q == d->out && (d->q_st == d->o_st || d->seqs.n_tok == 1)) && vlt5_rows_overlap(out, q)) return VLT5_ERR_ARG;
+    if (vlt5_rows_overlap(out, {c.k, c.n_pages, cache, cache}) || vlt5_rows_overlap(out, {c.v, c.n_pages, cache, cache})) return VLT5_ERR_ARG;
     if (d->seqs.n_tok == 0) return VLT5_OK;
     PagedAttnArgs a;
     a.s = vlt5_paged_seqs_of(&c, &d->seqs);

@@ -552,7 +552,8 @@ def paged_attn(q, cache, table, kv_lens, *, cu_q=None, max_q=None, max_kv=None, 
 
     heads: any multiple of the cache's; scale > 0; causal: a token sees the positions up to its own, else all keys; rel_bias f32 [heads, n]: added by
     how far the key lies back, its last column for everything further (T5's decoder bias); max_kv: about the longest length, for the split
-    of the work only.  A token that sees no key gets zeros; rows of `out` that belong to no sequence keep what they hold.
+    of the work only.  A token that sees no key gets zeros; rows of `out` that belong to no sequence keep what they hold.  `out` may be
+    `q` itself and otherwise shares no memory with it.
     Returns out bf16 [tokens, heads * d_kv], with want_lse also f32 [tokens, heads] (-inf without keys)."""
     dev = q.device
     at, st = _here(q)
