@@ -739,8 +739,8 @@ int vlt5_kv_page_read(const vlt5_paged_kv* c, const vlt5_paged_seqs* q, int T, v
  * key that lies `dist` positions back, the last entry for every larger dist -- T5's bucketed bias of a decoder as a function of the
  * distance.  A token that sees no key gets zeros and lse -inf.  What lies behind a sequence's last key may hold anything.  A key masked by
  * `causal` may too; so may its value as vlt5_kv_page_write leaves it in the 8-bit types, but a bf16 VALUE that is not finite reaches every
- * token that shares a tile of keys with it.  lse (optional) f32 [n_tok][H].  max_kv: about the longest kv_lens (0 = the table's width); it
- * only decides how the work is split.  workspace: vlt5_paged_attn_workspace_bytes of the same desc (0: none needed, always so where max_kv
+ * token that shares a tile of keys with it.  lse (optional) f32 [n_tok][H].  max_kv: about the longest kv_lens (0, or more than the
+ * table's width = that width); it only decides how the work is split.  workspace: vlt5_paged_attn_workspace_bytes of the same desc (0: none needed, always so where max_kv
  * or the table's width is below VLT5_PAGED_SHARED_KV), 16-byte aligned, one per call in flight. */
 #define VLT5_PAGED_SHARED_KV 1024
 typedef struct {

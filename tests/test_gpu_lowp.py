@@ -810,3 +810,12 @@ def test_attention_in_the_place_of_its_queries(dev, ops, new, lens):
         flat = torch.zeros(n + 1, 256, device=dev, dtype=BF)
         with pytest.raises(Vlt5Error):
             ops.paged_attn(flat[:n], c, *args, out=flat[1:], **kw)
+
+
+@pytest.mark.parametrize("max_kv", [-3, 1, 900, 5000, 2 ** 31 - 1])
+@pytest.mark.parametrize("lens", [[600], [1500]])
+def test_any_max_kv_is_taken(dev, ops, max_kv, lens):
+    """Shorter and longer than the table, which is what a sequence can have: a hint for the split."""
+    c, table = make_cache(ops, dev, lens, 2, 64, 16, FP8, seed=38)
+    for new in ([1], [50]):
+        check_attn(ops, dev, c, table, new, lens, 4, max_kv=max_kv, seed=1)

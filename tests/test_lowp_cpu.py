@@ -178,3 +178,17 @@ def test_attention_over_its_own_queries_is_refused(built):
                    dict(out=M + 2 * 512 + 496), dict(out=2 * M + 4 * 2 * 16 * 64 - 16), dict(out=3 * M - 2 * 512 - 16)):
         d = built.PagedAttnDesc(**{**dict(kv=kv, seqs=seq, q=M, q_st=256, o_st=256, H=4, scale=1.0, causal=1), **change})
         assert f(C.byref(d), None) == ARG, change
+
+
+def test_max_kv_past_the_table_counts_as_the_table(built):
+    """No sequence can have more keys than its table: below VLT5_PAGED_SHARED_KV of them a call needs no workspace, whatever max_kv says."""
+    size, most = built.lib().vlt5_paged_attn_workspace_bytes, built.PAGED_SHARED_KV
+
+    def need(max_pages, max_kv, n_tok=1, H=4):
+        return size(C.byref(built.PagedAttnDesc(kv=built.PagedKV(**KV), seqs=built.PagedSeqs(**{**SEQ, "B": 1, "n_tok": n_tok, "cu_q": P, "max_q": n_tok, "max_pages": max_pages}), q=P, q_st=256,
+                                                out=P, o_st=256, H=H, scale=1.0, causal=1, max_kv=max_kv)))
+    for n_tok in (1, 40, 700):
+        for max_kv in (0, 1, most, 5000, 1 << 30):
+            assert need(most // 16 - 1, max_kv, n_tok) == 0, (n_tok, max_kv)
+            assert need(most // 16, max_kv, n_tok) == (0 if max_kv == 1 else need(most // 16, 0, n_tok)) and need(most // 16, 0, n_tok) > 0
+            assert need(4096, max_kv, n_tok) >= need(most // 16, max_kv, n_tok)

@@ -799,7 +799,7 @@ struct PagedPlan { int chunk, row_tiles, splits, waves, tiles; };              /
 PagedPlan paged_plan(const vlt5_paged_attn_desc* d, const PagedSeqs& s) {
     const int g = d->H / d->kv.n_kv_heads;
     const long long rows = (long long)s.max_q * g, pairs = (long long)s.B * d->kv.n_kv_heads;
-    const long long most_kv = d->max_kv > 0 ? d->max_kv : (long long)d->seqs.max_pages * d->kv.page_size;
+    const long long width = (long long)d->seqs.max_pages * d->kv.page_size, most_kv = d->max_kv > 0 && d->max_kv < width ? d->max_kv : width;
     auto share = [&](long long n, int parts) {                                 // ... of the keys between n workgroups, at least 1024 / parts for one
         const long long most = most_kv < VLT5_PAGED_SHARED_KV ? 1 : most_kv / (VLT5_PAGED_SHARED_KV / parts);
         n = n < most ? n : most;

@@ -582,7 +582,7 @@ def paged_attn(q, cache, table, kv_lens, *, cu_q=None, max_q=None, max_kv=None, 
         desc = L.PagedAttnDesc(kv, seqs, q.data_ptr(), _row_stride(q, n, width), out.data_ptr(), o_st, None if lse is None else lse.data_ptr(), bias, nd, H, scale,
                                causal, max_kv or 0, None, 0)
         ref = C.byref(desc)
-        if (max_kv or seqs.max_pages * kv.page_size) >= L.PAGED_SHARED_KV:           # (below, the keys of a row are not shared out)
+        if seqs.max_pages * kv.page_size >= L.PAGED_SHARED_KV and not 0 < desc.max_kv < L.PAGED_SHARED_KV:      # (below, the keys of a row are not shared out)
             need = l.vlt5_paged_attn_workspace_bytes(ref)
             if need > 0:
                 ws = torch.empty(need, device=dev, dtype=torch.uint8)
