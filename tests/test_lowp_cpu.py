@@ -192,3 +192,17 @@ def test_max_kv_past_the_table_counts_as_the_table(built):
             assert need(most // 16 - 1, max_kv, n_tok) == 0, (n_tok, max_kv)
             assert need(most // 16, max_kv, n_tok) == (0 if max_kv == 1 else need(most // 16, 0, n_tok)) and need(most // 16, 0, n_tok) > 0
             assert need(4096, max_kv, n_tok) >= need(most // 16, max_kv, n_tok)
+
+
+def test_more_threads_than_a_grid_holds_are_refused(built):
+    """A grid's threads are counted in 32 bits; without max_q it has room for every token in every sequence."""
+    L = built.lib()
+    kv = built.PagedKV(**{**KV, "n_kv_heads": 1024})
+    many = built.PagedSeqs(**{**SEQ, "B": 65535, "n_tok": 65535, "max_pages": 16})
+    d = dict(kv=kv, q=P, q_st=65536, out=1 << 44, o_st=65536, H=1024, scale=1.0, causal=1)
+    assert L.vlt5_paged_attn(C.byref(built.PagedAttnDesc(seqs=many, **d)), None) == ARG
+    kv = built.PagedKV(**{**KV, "n_kv_heads": 16, "d_kv": 128})
+    long = built.PagedSeqs(**{**SEQ, "cu_q": P, "n_tok": 1 << 27, "max_q": 0})
+    assert L.vlt5_kv_page_write(C.byref(kv), C.byref(long), P, 2048, P, 2048, None) == ARG
+    assert L.vlt5_kv_page_read(C.byref(kv), C.byref(long), 1 << 27, P, P, None) == ARG
+    assert L.vlt5_quant_w4(P, None, 1 << 20, 1 << 16, 1 << 20, 32, P, P, None) == ARG

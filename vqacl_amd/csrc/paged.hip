@@ -7,6 +7,7 @@
 //
 // Both kernels move bytes and nothing else: bound by memory.
 #include "paged.h"
+#include "rows.h"
 
 namespace {
 
@@ -189,7 +190,7 @@ extern "C" int vlt5_kv_page_write(const vlt5_paged_kv* c, const vlt5_paged_seqs*
     const PagedSeqs s = vlt5_paged_seqs_of(c, q);
     const long long rows = ((long long)s.max_q + RPT - 1) / RPT * 2 * c->n_kv_heads;
     const long long blocks = (rows * (c->d_kv / 8) + 255) / 256;
-    if (blocks > 0x7fffffffLL) return VLT5_ERR_ARG;
+    if (blocks * 256 > VLT5_MOST_THREADS) return VLT5_ERR_ARG;
     const dim3 grid((unsigned)blocks, s.B);
 #define KVW(T, D) hipLaunchKernelGGL((kv_write_kernel<T, D>), grid, dim3(256), 0, (hipStream_t)stream, s, (const bf16_t*)k, k_st, (const bf16_t*)v, v_st, \
                                      (unsigned char*)c->k, (unsigned char*)c->v, c->k_scale, c->v_scale, c->n_kv_heads)
@@ -207,7 +208,7 @@ extern "C" int vlt5_kv_page_read(const vlt5_paged_kv* c, const vlt5_paged_seqs* 
     if (T == 0) return VLT5_OK;
     const PagedSeqs s = vlt5_paged_seqs_of(c, q);
     const long long blocks = (((long long)T + RPT - 1) / RPT * 2 * c->n_kv_heads * (c->d_kv / 8) + 255) / 256;
-    if (blocks > 0x7fffffffLL) return VLT5_ERR_ARG;
+    if (blocks * 256 > VLT5_MOST_THREADS) return VLT5_ERR_ARG;
     const dim3 grid((unsigned)blocks, s.B);
 #define KVR(TY, D) hipLaunchKernelGGL((kv_read_kernel<TY, D>), grid, dim3(256), 0, (hipStream_t)stream, s, (const unsigned char*)c->k, (const unsigned char*)c->v, \
                                       c->k_scale, c->v_scale, c->n_kv_heads, T, (bf16_t*)k_out, (bf16_t*)v_out)

@@ -865,7 +865,7 @@ extern "C" int vlt5_paged_attn(const vlt5_paged_attn_desc* d, void* stream) {
     const long long tiles = (long long)a.s.B * a.Hkv * a.row_tiles;
     const int wpr = a.splits > 8 ? 4 : 1;                                           // waves that join a row
     const long long joins = ((long long)a.s.B * a.H * a.s.max_q * wpr + 3) / 4;
-    if (tiles * a.splits > 0x7fffffffLL || joins > 0x7fffffffLL) return VLT5_ERR_ARG;
+    if (tiles * a.splits * (64 * plan.waves) > VLT5_MOST_THREADS || joins * 256 > VLT5_MOST_THREADS) return VLT5_ERR_ARG;
     hipStream_t st = (hipStream_t)stream;
     int lrc = VLT5_OK;
 #define PA(T, D) do { if (plan.chunk && plan.waves == 8) lrc = a.bias ? chunk_launch<T, D, true, 2>(a, (unsigned)(tiles * a.splits), st) : chunk_launch<T, D, false, 2>(a, (unsigned)(tiles * a.splits), st); \

@@ -1,6 +1,9 @@
-// Host side: do two sets of rows share a byte?  Used where an output over an input would let one workgroup write what another has yet to read.
+// Host side: what a call is refused for before it is launched.
 #pragma once
 
+#define VLT5_MOST_THREADS 0xffffffffLL                   // of a grid in one dimension: the runtime counts them in 32 bits
+
+// Do two sets of rows share a byte?  Asked where an output over an input would let one workgroup write what another has yet to read.
 // n rows of `width` bytes, `stride` bytes apart (of one row the stride does not matter); rows of one set do not overlap each other
 struct RowSpan {
     const void* at; long long n, stride, width;

@@ -459,7 +459,7 @@ extern "C" int vlt5_quant_w4(const float* w_f32, const void* w_bf16, long long l
     if ((K & 31) || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 1)) return VLT5_ERR_ALIGN;
     const int groups = (K + group - 1) / group;
     const long long blocks = ((long long)N * groups * (group / 8) + 255) / 256;
-    if (blocks > 0x7fffffffLL) return VLT5_ERR_ARG;
+    if (blocks * 256 > VLT5_MOST_THREADS) return VLT5_ERR_ARG;
     hipStream_t st = (hipStream_t)stream;
 #define QW4(G) hipLaunchKernelGGL(quant_w4_kernel<G>, dim3((unsigned)blocks), dim3(256), 0, st, w_f32, (const bf16_t*)w_bf16, ldw, N, K, groups, (uint32_t*)codes, (bf16_t*)scales)
     if (group == 32) QW4(32);
