@@ -737,11 +737,11 @@ int vlt5_kv_page_read(const vlt5_paged_kv* c, const vlt5_paged_seqs* q, int T, v
  * `out` may be `q` (the same rows); over q in any other way, or over the cache, it is refused.
  * causal: a token sees the positions up to its own, else all kv_lens[b].  rel_bias f32 [H][n_dist] (causal only): added to the score of a
  * key that lies `dist` positions back, the last entry for every larger dist -- T5's bucketed bias of a decoder as a function of the
- * distance.  A token that sees no key gets zeros and lse -inf.  What lies behind a sequence's last key may hold anything.  A key masked by
- * `causal` may too; so may its value as vlt5_kv_page_write leaves it in the 8-bit types, but a bf16 VALUE that is not finite reaches every
- * token that shares a tile of keys with it.  lse (optional) f32 [n_tok][H].  max_kv: about the longest kv_lens (0, or more than the
- * table's width = that width); it only decides how the work is split.  workspace: vlt5_paged_attn_workspace_bytes of the same desc (0: none needed, always so where max_kv
- * or the table's width is below VLT5_PAGED_SHARED_KV), 16-byte aligned, one per call in flight. */
+ * distance.  A token that sees no key gets zeros and lse -inf.  What a token does not see may hold anything: keys behind the last one, and
+ * keys that `causal` masks, whose values, finite or not, reach only the tokens that see them (an 8-bit value whose scale is not finite shows
+ * in all of a token that sees it).  lse (optional) f32 [n_tok][H].  max_kv: about the longest kv_lens (0, or more than the table's width =
+ * that width); it only decides how the work is split.  workspace: vlt5_paged_attn_workspace_bytes of the same desc (0: none needed, always
+ * so where max_kv or the table's width is below VLT5_PAGED_SHARED_KV), 16-byte aligned, one per call in flight. */
 #define VLT5_PAGED_SHARED_KV 1024
 typedef struct {
     vlt5_paged_kv kv; vlt5_paged_seqs seqs;

@@ -819,3 +819,61 @@ def test_any_max_kv_is_taken(dev, ops, max_kv, lens):
     c, table = make_cache(ops, dev, lens, 2, 64, 16, FP8, seed=38)
     for new in ([1], [50]):
         check_attn(ops, dev, c, table, new, lens, 4, max_kv=max_kv, seed=1)
+
+
+@pytest.mark.parametrize("kind", [BF, FP8])
+@pytest.mark.parametrize("d,g,new,lens,nd", [
+    (64, 1, [20], [50], 0), (128, 3, [21, 9], [40, 70], 0), (64, 2, [70], [90], 40), (128, 1, [130], [330], 0), (64, 4, [150, 60], [150, 300], 0), (128, 4, [40], [2600], 16), (64, 16, [4], [1500], 0), (128, 3, [5], [29], 0), (64, 40, [4], [60], 0),
+])
+def test_a_value_that_is_not_finite_is_seen_by_later_tokens_only(dev, ops, kind, d, g, new, lens, nd):
+    """Values of the cache that are infinite or NaN (e4m3: NaN) show in their column, in the tokens that see them, and nowhere else."""
+    hk = 2
+    c, table = make_cache(ops, dev, lens, hk, d, 16, kind, seed=d + g)
+    n = sum(new)
+    q = torch.randn(n, hk * g * d, generator=gen(n)).to(BF).to(dev)
+    bias = None if not nd else torch.randn(hk * g, nd, generator=gen(nd)).to(dev)
+    args, kw = (table.to(dev), ints(dev, lens)), dict(cu_q=ints(dev, starts(new)), max_q=max(new), scale=0.1, rel_bias=bias)
+    clean, lse = ops.paged_attn(q, c, *args, want_lse=True, **kw)
+    want = clean.float().view(n, hk, g, d).clone()
+    marks = []                                                                              # sequence, position, head, column, value
+    for b in range(len(new)):
+        p0 = lens[b] - new[b]
+        marks += [(b, p0 + new[b] // 2, 0, 5, math.nan), (b, p0 + new[b] // 3, 1, d - 1, math.inf), (b, p0 + new[b] // 3, 1, 7, math.inf), (b, lens[b] - 1, 1, 7, -math.inf),
+                  (b, p0 + 1, 0, 0, -math.inf), (b, lens[b] - 2, 0, d // 2, math.inf)]
+    for b, pos, h, col, x in marks:
+        p, r = int(table[b, pos // 16]), pos % 16
+        if kind == BF:
+            c.v[p, h, r, col] = x
+        else:
+            raw(c.v)[p, h, r, col] = 0x7f if x > 0 else 0xff
+            x = math.nan
+        seen = slice(starts(new)[b] + pos - (lens[b] - new[b]), starts(new)[b + 1])
+        want[seen, h, :, col] = want[seen, h, :, col].masked_fill(torch.isfinite(want[seen, h, :, col]), 0) + x
+    for _ in range(2):
+        got, l2 = ops.paged_attn(q, c, *args, want_lse=True, **kw)
+        got = got.float().view(n, hk, g, d)
+        wrong = int((torch.isnan(got) != torch.isnan(want)).sum()), int((torch.isinf(got) != torch.isinf(want)).sum()), int((l2 != lse).sum())
+        assert wrong == (0, 0, 0)
+        odd = ~torch.isfinite(want)
+        assert torch.equal(got.masked_fill(odd, 0), want.masked_fill(odd, 0))                # the rest as without them
+        assert torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
+    assert bool(torch.isnan(want).any()) and (kind == FP8 or bool(torch.isinf(want).any()))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_the_first_of_several_tokens_does_not_see_the_others(dev, ops, kind):
+    """max_q = 1: the one token that is processed is not the sequence's last, and what the others left is not its."""
+    lens, new = [40, 70], [3, 9]
+    c, table = make_cache(ops, dev, lens, 2, 64, 16, kind, seed=41)
+    q = torch.randn(12, 512, generator=gen(8)).to(BF).to(dev)
+    args, kw = (table.to(dev), ints(dev, lens)), dict(cu_q=ints(dev, [0, 3, 12]), scale=0.1)
+    want = ops.paged_attn(q, c, *args, **kw)[[0, 3]]
+    for b in range(2):
+        for pos in range(lens[b] - new[b] + 1, lens[b]):
+            p, r = int(table[b, pos // 16]), pos % 16
+            for pages, scales in ((c.k, c.k_scale), (c.v, c.v_scale)):
+                raw(pages)[p, :, r] = math.nan if kind == BF else 127
+                if scales is not None:
+                    scales[p, :, r] = math.nan
+    got = ops.paged_attn(q, c, *args, max_q=1, **kw)[[0, 3]]
+    assert torch.equal(got, want)

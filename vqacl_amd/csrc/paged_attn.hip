@@ -68,6 +68,42 @@ __device__ __forceinline__ uint32_t vpair(const VRow<T, DK>& a, const VRow<T, DK
     }
 }
 
+// Values that are not finite.  A masked probability of 0 times such a value is not 0, so where some rows of a workgroup see a key that others do not
+// (causal, the last keys), they are taken out of V on its way into the product (bf16 and e4m3; an int8 value is always finite), and the first
+// position of +inf and of -inf is kept for each d (a NaN counts as both): with the mask a row sees that position or it sees none of them, so the
+// row's output gains +inf, -inf or both, which is NaN, at the end.  Elsewhere every row sees the key and the product gives what it gives.
+// It costs a look at the values of the last tiles and a barrier: 8 x 16 tokens over 500 bf16 keys, 12 heads of 64, 8.1 -> 8.8 us, 8 x 5 over 3000, 32 / 8
+// of 128, 32.4 -> 34.9, 45 x 79 over 79 11.6 -> 12.0, 1 x 1000 over 8000 98.1 -> 98.3.
+struct OddValues {                                     // in LDS: first position of +inf by d, of -inf by d (or MOST), are there any?
+    int* at; int dk;
+    static constexpr int MOST = 0x7fffffff;
+    __device__ __forceinline__ void clear(int tid, int threads) const {
+        for (int i = tid; i < 2 * dk + 1; i += threads) at[i] = i < 2 * dk ? MOST : 0;
+    }
+    __device__ __forceinline__ bool any() const { return __builtin_amdgcn_readfirstlane(at[2 * dk]); }
+    __device__ __forceinline__ float add(int d, int len) const { return (at[d] < len ? INFINITY : 0.f) + (at[dk + d] < len ? -INFINITY : 0.f); }
+};
+template <int T>
+__device__ __forceinline__ bool odd_values(uint32_t w) {   // any in a raw dword?
+    if constexpr (T == VLT5_KV_BF16) return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+    else if constexpr (T == VLT5_KV_FP8) return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    else return false;
+}
+// takes them out of a raw dword that holds d, d + 1, .. of the key at `pos`
+template <int T>
+__device__ __forceinline__ void take_odd(uint32_t& w, const OddValues& o, int d, int pos) {
+    constexpr int BITS = 8 * KvType<T>::BYTES;
+    for (int i = 0; i < 32 / BITS; ++i) {
+        const uint32_t x = w >> (i * BITS) & (0xffffffffu >> (32 - BITS)), mag = T == VLT5_KV_BF16 ? x & 0x7fffu : x & 0x7fu;
+        if (mag < (T == VLT5_KV_BF16 ? 0x7f80u : 0x7fu)) continue;
+        const bool nan = T == VLT5_KV_FP8 || mag > 0x7f80u;
+        if (nan || x == mag) atomicMin(o.at + d + i, pos);
+        if (nan || x != mag) atomicMin(o.at + o.dk + d + i, pos);
+        o.at[2 * o.dk] = 1;
+        w &= ~((0xffffffffu >> (32 - BITS)) << (i * BITS));
+    }
+}
+
 // The raw rows of 32 keys, as one lane holds them: for the scores keys 16 i + lane % 16 (16-byte pieces of the row), for the output the rows
 // 16 i + 4 * (lane / 16) + 0 .. 3, DK / 16 values of each.
 template <int T, int DK>
@@ -96,7 +132,9 @@ struct KeyStep {
 
 // NW waves share the keys of 16 R rows in steps of 32, the next step's rows on their way while one is used; the page ids of a wave's next 32 steps
 // come with one load, two to a step.  The R row tiles use the same operands of K and V: a key is read and converted once for all of them.
-template <int T, int DK, int NW, int R>
+// ODD: a causal call of several tokens a sequence, whose last keys some of its rows do not see (single tokens see all: without the code for it three
+// waves of the 64-wide form fit a SIMD, with it two).
+template <int T, int DK, int NW, int R, bool ODD>
 __global__ __launch_bounds__(NW * 64, R * DK > 128 ? 1 : 2) void paged_attn_kernel(const PagedAttnArgs a) {
     constexpr int NF = DK / 32, ND = DK / 16;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, kq = lane >> 4;
@@ -138,6 +176,10 @@ __global__ __launch_bounds__(NW * 64, R * DK > 128 ? 1 : 2) void paged_attn_kern
 #pragma unroll
         for (int f = 0; f < NF; ++f) fq[i][f] = *reinterpret_cast<const bf16x8_t*>(qrow + (T == VLT5_KV_BF16 ? f * 32 + kq * 8 : (f >> 1) * 64 + kq * 16 + (f & 1) * 8));
     }
+    __shared__ int first_odd[ODD ? 2 * DK + 1 : 1];
+    const OddValues odd = {first_odd, DK};
+    const bool track = ODD && first != last;
+    if (track) odd.clear(threadIdx.x, NW * 64);
     __shared__ float sb[BIAS_LDS];
     const bool near_lds = a.bias && a.g * a.nd <= BIAS_LDS;
     const float* bias = a.bias ? a.bias + (size_t)hk * a.g * a.nd : nullptr;
@@ -266,13 +308,33 @@ __global__ __launch_bounds__(NW * 64, R * DK > 128 ? 1 : 2) void paged_attn_kern
             }
             fp[q] = __builtin_bit_cast(bf16x8_t, make_uint4(pb[0][0], pb[0][1], pb[1][0], pb[1][1]));
         }
-        if (!whole) {                                                              // what lies behind the last key may hold anything, NaN too
+        if (!whole) {                                                              // what lies behind the last key that a row sees may hold anything, NaN too
             asm volatile("");
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (!(pg[buf][i] >= 0 && t0 + i * 16 + kq * 4 + e < sq.len)) x.v[i][e] = VRow<T, DK>{};
+                    if (!(pg[buf][i] >= 0 && t0 + i * 16 + kq * 4 + e < Lmax)) x.v[i][e] = VRow<T, DK>{};
+            if (track) {
+                bool any = false;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (uint32_t v : x.v[i][e].w) any |= odd_values<T>(v);
+                if (__builtin_expect(any, 0)) {
+                    int me = threadIdx.x;
+                    asm volatile("" : "+v"(me));                                   // (what follows is formed here: kept since the start it would spill)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int n = 0; n < (int)(sizeof x.v[i][e].w / 4); ++n)
+                                take_odd<T>(x.v[i][e].w[n], odd, me % 16 * ND + n * 4 / KvType<T>::BYTES, t0 + i * 16 + me / 16 % 4 * 4 + e);
+                }
+            }
         }
 #pragma unroll
         for (int j = 0; j < ND; ++j) {
@@ -294,8 +356,8 @@ __global__ __launch_bounds__(NW * 64, R * DK > 128 ? 1 : 2) void paged_attn_kern
         for (int k = 0; k < 2; ++k)
             if ((int)threadIdx.x + k * NW * 64 < a.g * a.nd) sb[threadIdx.x + k * NW * 64] = table[k];
         for (int k = threadIdx.x + 2 * NW * 64; k < a.g * a.nd; k += NW * 64) sb[k] = bias[k];
-        __syncthreads();
     }
+    if (near_lds || track) __syncthreads();
     int i = 0;
     for (; i + 2 < mine; i += 2) {                                                 // (every load unconditional, or the waits could not be counted)
         load(i + 1, 1);                                                            // (i is even: never the first of 32 steps)
@@ -344,6 +406,10 @@ __global__ __launch_bounds__(NW * 64, R * DK > 128 ? 1 : 2) void paged_attn_kern
                 const float4 x = *reinterpret_cast<const float4*>(&so[ww][rr][d]);
                 sum += sl[ww][rr] * f;
                 acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
+            }
+            if (track && odd.any()) {
+                const int len = min(p0 + r / a.g + 1, sq.len);
+                acc.x += odd.add(d, len); acc.y += odd.add(d + 1, len); acc.z += odd.add(d + 2, len); acc.w += odd.add(d + 3, len);
             }
             const int hh = hk * a.g + r % a.g;
             const size_t token = (size_t)(sq.q0 + r / a.g);
@@ -399,6 +465,10 @@ __global__ __launch_bounds__(256 * KS, DK == 64 && KS == 1 ? 3 : 2) void paged_c
     const int Lmax = max(a.causal ? p0 + min(rt * 128 + 127, rows - 1) / a.g + 1 : sq.len, 0);
     const int wLmin = a.causal ? p0 + min(wr0, rows - 1) / a.g + 1 : sq.len;            // the wave's rows all see the keys below this ...
     const int wLmax = wr0 < rows ? (a.causal ? p0 + min(wr0 + 31, rows - 1) / a.g + 1 : sq.len) : 0;      // ... and none those from here on
+    const bool track = T != VLT5_KV_INT8 && a.causal;
+    const int least = p0 + rt * 128 / a.g + 1;                                          // the workgroup's rows do not all see the keys from here on
+    const OddValues odd = {reinterpret_cast<int*>(smem + 2 * KS * BUF + (BIAS ? CHUNK_BIAS_LDS * 4 : 0)), DK};
+    if (track) odd.clear(tid, 256 * KS);
     const int per = ((Lmax + a.splits - 1) / a.splits + 63) & ~63;
     const int lo = min(sp * per, Lmax), hi = min(lo + per, Lmax);
 
@@ -482,7 +552,23 @@ __global__ __launch_bounds__(256 * KS, DK == 64 && KS == 1 ? 3 : 2) void paged_c
                     for (int i = 0; i < VW; ++i) vr[e][i] = 0;
         }
     };
-    auto stage = [&](char* buf) {
+    auto stage = [&](char* buf, int tile) {
+        if (track && lo + tile * 64 + 64 > least) {
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int i = 0; i < VW; ++i) any |= odd_values<T>(vr[e][i]);
+            if (__builtin_expect(any, 0)) {
+                int me = tid;
+                asm volatile("" : "+v"(me));
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+#pragma unroll
+                    for (int i = 0; i < VW; ++i)
+                        take_odd<T>(vr[e][i], odd, me % 32 * NT + i * 4 / BY, lo + tile * 64 + w4 * 16 + (e >> 2) * 8 + me / 32 % 2 * 4 + (e & 3));
+            }
+        }
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
             char* p = buf + ((i * 256 + w4 * 64) / KCH + lane / KCH) * KROW + (lane % KCH) * (16 / BY * 2);
@@ -533,7 +619,8 @@ __global__ __launch_bounds__(256 * KS, DK == 64 && KS == 1 ? 3 : 2) void paged_c
             if (tid + j * 256 * KS < entries) sb[tid + j * 256 * KS] = table[j];
         for (int i = tid + 512 * KS; i < entries; i += 256 * KS) sb[i] = entry(i);
     }
-    if (half < tiles) stage(mine);
+    if (track) __syncthreads();
+    if (half < tiles) stage(mine, half);
     __syncthreads();
     for (int turn = 0; turn * KS < tiles; ++turn) {
         const int tile = turn * KS + half, t0 = lo + tile * 64, cur = turn & 1;
@@ -653,7 +740,7 @@ __global__ __launch_bounds__(256 * KS, DK == 64 && KS == 1 ? 3 : 2) void paged_c
                 for (int j = 0; j < NT; ++j)
                     o[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(v + ((g2 * NT + j) * 64 + lane) * 16), fp[g2], o[j], 0, 0, 0);
         }
-        if (more) stage(mine + (cur ^ 1) * BUF);
+        if (more) stage(mine + (cur ^ 1) * BUF, tile + KS);
         __syncthreads();
     }
     l += __shfl_xor(l, 32, 64);
@@ -680,6 +767,12 @@ __global__ __launch_bounds__(256 * KS, DK == 64 && KS == 1 ? 3 : 2) void paged_c
             for (int e = 0; e < 16; ++e) o[j][e] = o[j][e] * f0 + x[(j * 16 + e) * 64] * f1;
     }
     if (wr0 + r32 >= rows) return;
+    if (track && odd.any()) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[j][e] += odd.add(NT * (e / 4 * 8 + h * 4 + e % 4) + j, L);
+    }
     const float mnat = BIAS ? m : m * a.scale;
     const size_t row = (size_t)(sq.q0 + tok) * a.H + hq;
     if (a.splits == 1) {
@@ -763,16 +856,21 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
     if (a.lse && lane == 0) a.lse[row] = sum == 0.f ? -INFINITY : mx + logf(sum);
 }
 
+template <int T, int DK, bool ODD>
+void rows_launch(const PagedAttnArgs& a, unsigned blocks, int waves, int tiles, hipStream_t st) {
+    if (waves == 1) hipLaunchKernelGGL((paged_attn_kernel<T, DK, 1, 1, ODD>), dim3(blocks), dim3(64), 0, st, a);
+    else if (tiles == 1) hipLaunchKernelGGL((paged_attn_kernel<T, DK, 4, 1, ODD>), dim3(blocks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((paged_attn_kernel<T, DK, 4, 2, ODD>), dim3(blocks), dim3(256), 0, st, a);
+}
 template <int T, int DK>
 void rows_launch(const PagedAttnArgs& a, unsigned blocks, int waves, int tiles, hipStream_t st) {
-    if (waves == 1) hipLaunchKernelGGL((paged_attn_kernel<T, DK, 1, 1>), dim3(blocks), dim3(64), 0, st, a);
-    else if (tiles == 1) hipLaunchKernelGGL((paged_attn_kernel<T, DK, 4, 1>), dim3(blocks), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((paged_attn_kernel<T, DK, 4, 2>), dim3(blocks), dim3(256), 0, st, a);
+    if (T != VLT5_KV_INT8 && a.causal && a.s.max_q > 1) rows_launch<T, DK, T != VLT5_KV_INT8>(a, blocks, waves, tiles, st);
+    else rows_launch<T, DK, false>(a, blocks, waves, tiles, st);
 }
 template <int T, int DK, bool BIAS, int KS>
 int chunk_launch(const PagedAttnArgs& a, unsigned blocks, hipStream_t st) {
     static std::atomic<unsigned long long> done{0};
-    constexpr int bytes = 2 * KS * (64 * (DK * 2 + 16) + 4 * (DK / 32) * 1024 + 512) + (BIAS ? CHUNK_BIAS_LDS * 4 : 0);
+    constexpr int bytes = 2 * KS * (64 * (DK * 2 + 16) + 4 * (DK / 32) * 1024 + 512) + (BIAS ? CHUNK_BIAS_LDS * 4 : 0) + (T == VLT5_KV_INT8 ? 0 : 8 * DK + 16);
     const int rc = vlt5_lds_optin((const void*)paged_chunk_kernel<T, DK, BIAS, KS>, bytes, done);
     if (rc) return rc;
     hipLaunchKernelGGL((paged_chunk_kernel<T, DK, BIAS, KS>), dim3(blocks), dim3(256 * KS), bytes, st, a);
