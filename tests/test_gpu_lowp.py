@@ -824,6 +824,7 @@ def test_any_max_kv_is_taken(dev, ops, max_kv, lens):
 @pytest.mark.parametrize("kind", [BF, FP8])
 @pytest.mark.parametrize("d,g,new,lens,nd", [
     (64, 1, [20], [50], 0), (128, 3, [21, 9], [40, 70], 0), (64, 2, [70], [90], 40), (128, 1, [130], [330], 0), (64, 4, [150, 60], [150, 300], 0), (128, 4, [40], [2600], 16), (64, 16, [4], [1500], 0), (128, 3, [5], [29], 0), (64, 40, [4], [60], 0),
+    (64, 1, [131] * 66, [131 + 3 * b for b in range(66)], 0), (64, 1, [131] * 66, [131 + 3 * b for b in range(66)], 30), (128, 1, [131] * 66, [131 + 3 * b for b in range(66)], 0),
 ])
 def test_a_value_that_is_not_finite_is_seen_by_later_tokens_only(dev, ops, kind, d, g, new, lens, nd):
     """Values of the cache that are infinite or NaN (e4m3: NaN) show in their column, in the tokens that see them, and nowhere else."""
@@ -877,3 +878,32 @@ def test_the_first_of_several_tokens_does_not_see_the_others(dev, ops, kind):
                     scales[p, :, r] = math.nan
     got = ops.paged_attn(q, c, *args, max_q=1, **kw)[[0, 3]]
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("causal,g,nd", [(True, 1, 0), (True, 1, 40), (True, 2, 300), (False, 1, 0)])
+def test_chunks_on_a_full_chip(dev, ops, kind, d, causal, g, nd):
+    """More tiles of 128 rows than CUs: four waves a workgroup, which read all of its keys; two row tiles a sequence, one sequence whose page ids
+    are loaded twice (more than 16 tiles of 64 keys), one with a page that is not there, one that is empty and one with one token."""
+    B, hk = 17, 8
+    news = [140 - 4 * b for b in range(B)]
+    lens = [n + (31 * b) % 90 for b, n in enumerate(news)]
+    lens[2] = 1150
+    news[5] = lens[5] = 0
+    news[6] = 1
+    c, table = make_cache(ops, dev, lens, hk, d, 16, kind, seed=d + nd)
+    table[9, 3] = -1
+    assert -(-max(news) * g // 128) * B * hk > 256
+    bias = 2 * torch.randn(hk * g, nd, generator=gen(nd)) if nd else None
+    check_attn(ops, dev, c, table, news, lens, hk * g, causal=causal, bias=bias, seed=1)
+
+
+@pytest.mark.parametrize("g,nd", [(8, 64), (8, 65), (8, 128), (8, 129), (2, 512), (2, 513), (2, 832), (2, 833), (4, 256), (4, 257), (4, 320), (4, 321), (1, 1024), (1, 1025), (1, 1856), (1, 1857)])
+@pytest.mark.parametrize("new", [[1, 1], [5, 2], [90, 33]])
+def test_bias_tables_that_fit_lds_and_that_do_not(dev, ops, g, nd, new):
+    """Both sides of what either kernel keeps in LDS (1024 entries; 2048 with 192 of padding a head), contexts longer and shorter than the table."""
+    kind, d = KINDS[(g + nd + len(new) + new[0]) % 3], 64 if (nd + new[0]) % 4 < 2 else 128
+    lens = [nd + 150, max(new[1], min(nd // 2, 400))]
+    c, table = make_cache(ops, dev, lens, 2, d, 32, kind, seed=nd)
+    check_attn(ops, dev, c, table, new, lens, 2 * g, bias=2 * torch.randn(2 * g, nd, generator=gen(nd)), seed=1)
