@@ -206,3 +206,12 @@ def test_more_threads_than_a_grid_holds_are_refused(built):
     assert L.vlt5_kv_page_write(C.byref(kv), C.byref(long), P, 2048, P, 2048, None) == ARG
     assert L.vlt5_kv_page_read(C.byref(kv), C.byref(long), 1 << 27, P, P, None) == ARG
     assert L.vlt5_quant_w4(P, None, 1 << 20, 1 << 16, 1 << 20, 32, P, P, None) == ARG
+
+
+def test_every_source_is_built_without_packed_f32_instructions():
+    """Some forms of v_pk_add / mul / fma_f32 have given wrong results on this target now and then: the compiler is told to make none of them."""
+    lines = subprocess.check_output(["make", "-C", os.path.join(ROOT, "vqacl_amd", "csrc"), "-n", "-B", "all", "exp"], text=True).splitlines()
+    compiles = [line for line in lines if " -c " in line]
+    sources = [f for f in os.listdir(os.path.join(ROOT, "vqacl_amd", "csrc")) if f.endswith(".hip")]
+    assert len(compiles) == len(sources) + 1
+    assert all("-Xclang -target-feature -Xclang -packed-fp32-ops" in line for line in compiles)

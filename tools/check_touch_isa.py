@@ -28,7 +28,7 @@ def regs(tok):
 
 
 def isa_of(f):
-    return subprocess.run(["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", f"-I{ROOT}/include", f"-I{CSRC}", "-S", "--cuda-device-only",
+    return subprocess.run(["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", f"-I{ROOT}/include", f"-I{CSRC}", "-S", "--cuda-device-only", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                            os.path.join(CSRC, f), "-o", "-"] + sys.argv[1:], capture_output=True, text=True).stdout.splitlines()
 
 

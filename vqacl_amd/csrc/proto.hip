@@ -71,13 +71,16 @@ __global__ __launch_bounds__(256) void class_mean_kernel(const float* __restrict
     }
 }
 
+// t * old + (1 - t) * now with its two roundings spelt out: the separate kernels and the fused head agree bit for bit
+__device__ __forceinline__ float moving_mean(float t, float old, float now) { return fmaf(1.f - t, now, t * old); }
+
 // update_prototype, elementwise over max(CQ,CV) x d
 __global__ void proto_update_kernel(const float* __restrict__ curQ, const float* __restrict__ curV, const float* __restrict__ numQ,
                                     const float* __restrict__ numV, float* __restrict__ Qp, float* __restrict__ Vp,
                                     float* __restrict__ Qnum, float* __restrict__ Vnum, float* __restrict__ qmem, int qmem_init,
                                     int first, int task, float alpha, float beta, int CQ, int CV, int d) {
     const int i = blockIdx.x * blockDim.x + threadIdx.x;
-    if (i < CV * d) Vp[i] = first ? curV[i] : beta * Vp[i] + (1.f - beta) * curV[i];
+    if (i < CV * d) Vp[i] = first ? curV[i] : moving_mean(beta, Vp[i], curV[i]);
     if (i < CQ * d) {
         const int row = i / d;
         if (first) {
@@ -86,7 +89,7 @@ __global__ void proto_update_kernel(const float* __restrict__ curQ, const float*
             Qp[i] = curQ[i];
         } else {
             const float now = (row == task) ? 0.f : curQ[i];
-            float mem = qmem_init ? alpha * qmem[i] + (1.f - alpha) * now : now;
+            float mem = qmem_init ? moving_mean(alpha, qmem[i], now) : now;
             if (row == task) mem = curQ[i];         // the reference writes the current row through an alias of the memory
             qmem[i] = mem;
             Qp[i] = mem;
@@ -261,14 +264,14 @@ __global__ __launch_bounds__(256) void proto_row_kernel(HeadArgs a) {
             for (int e = 0; e < 4; ++e) {
                 const int i = cls * d + c + e;
                 if (!isQ) {
-                    P[c + e] = a.first ? cur[e] : a.beta * P[c + e] + (1.f - a.beta) * cur[e];
+                    P[c + e] = a.first ? cur[e] : moving_mean(a.beta, P[c + e], cur[e]);
                 } else if (a.first) {
                     if (a.task == 0 || cls == a.task) P[c + e] = cur[e];
                 } else if (a.task == 0) {
                     P[c + e] = cur[e];
                 } else {
                     const float now = (cls == a.task) ? 0.f : cur[e];
-                    float mem = a.qmem_init ? a.alpha * a.qmem[i] + (1.f - a.alpha) * now : now;
+                    float mem = a.qmem_init ? moving_mean(a.alpha, a.qmem[i], now) : now;
                     if (cls == a.task) mem = cur[e];
                     a.qmem[i] = mem;
                     P[c + e] = mem;
