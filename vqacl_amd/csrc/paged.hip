@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const PagedSeqs s, const u
                 const uint32_t p[4] = {p0.x, p0.y, p1.x, p1.y};
                 uint32_t r[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) r[e] = pack_bf16x2(__uint_as_float(p[e] << 16) * sc[j], __uint_as_float(p[e] & 0xffff0000u) * sc[j]);   // exact codes: one rounding
+                for (int e = 0; e < 4; ++e) r[e] = pack_bf16x2(__uint_as_float(p[e] << 16) * sc[j], __uint_as_float(p[e] & 0xffff0000u) * sc[j]);   // to f32, then to bf16
                 out[j] = make_uint4(r[0], r[1], r[2], r[3]);
             }
         }

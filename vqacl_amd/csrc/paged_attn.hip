@@ -11,9 +11,11 @@
 // 8-bit codes are exact in bf16; the scale of a key multiplies its score, the scale of a value its probability (in f32, before the one
 // rounding of the probabilities to bf16, which with the output's own is all the rounding there is below 32 bits).
 //
-// Single tokens are bound by the bytes of the cache: 32 x 16384 keys, 8 kv heads of 128, e4m3: 148 us = 5.5 TB/s; 1 x 131071, int8: 42 us =
-// 6.6 TB/s (a part of it from the last-level cache) and 4.6 us to join its 64 shares.  Long chunks are bound by the matrix and vector units
-// together (42 % and 41 % busy at the 1.8 GHz such a load runs at): 2048 tokens over 16384 bf16 keys, 32 heads of 128: 545-590 us = 875-945 TFLOP/s.
+// Single tokens are bound by the bytes of the cache: 32 x 8192 - 16384 keys, 8 kv heads of 128, e4m3: 148 - 151 us = 5.5 TB/s (of 6.2 that a kernel
+// which does nothing but read reaches); in bf16 at 16384 each 372 us = 5.8.  1 x 131071, int8: 59 - 63 us a call = 4.4 - 4.7 TB/s, 4.7 of them to join
+// its 64 shares (48 where the same cache is read again and again: the last-level cache holds a part of it); in bf16 105 us.  Long chunks are
+// bound by the matrix and vector units together (42 % and 41 % busy at the 1.8 GHz such a load runs at): 2048 tokens over 16384 keys, 32 heads of
+// 128, 545 - 590 us in bf16 = 875 - 945 TFLOP/s (the first dozen launches of a process 620 - 670), 577 in e4m3, 603 in int8.
 #include "paged.h"
 #include "rows.h"
 
@@ -428,7 +430,10 @@ __global__ __launch_bounds__(NW * 64, R * DK > 128 ? 1 : 2) void paged_attn_kern
 
 // Room for the chunk kernel's bias tables, one per head of the group: distances from -PAD on (keys past a row's own, masked) to PAD past the last
 // entry, so that a tile's 32 entries of a lane lie at fixed places from one address, with no index arithmetic and few registers: the 64-wide form
-// leaves a CU three workgroups instead of two (45 x 79 tokens over 79 keys, 12 heads, int8, 128 distances: 13.1 -> 10.8 us, 9.5 without a bias).
+// leaves a CU three workgroups instead of two (45 x 79 tokens over 79 keys, 12 heads, int8, 128 distances: 13.1 -> 10.8 us, 9.5 without a bias; all of
+// them 79 long 14.0, 12.3 without; two to six registers that only the end needs are put away in front of the loop for it).  Larger tables, as of seven
+// heads a group with 128 distances, are read from memory, which costs no more where heads share: 8 x 200 over 712, 32 / 4 heads of 64, int8, 64 distances (LDS) 34.0 us, 65 (memory) 32.0,
+// 128 36.2, none 28.4; with a head a group 1856 distances 22.5 and 1857 25.3.
 constexpr int CHUNK_BIAS_LDS = 2048, PAD = 96;
 
 // ---- chunks: many rows share the keys ------------------------------------------------------------------------------------------------
@@ -887,7 +892,7 @@ bool paged_heads_ok(const vlt5_paged_attn_desc* d) {
 //   8000 152 -> 124, 41 x 40 over 10130 198 -> 182; a chip that is not full loses: 20 x 33 over 600 9.9 -> 12.3), in a bf16 cache, which has nothing
 //   to convert, from 33 on through LDS (4 x 40 over 20000 81 -> 71, 100 x 33 over 400 36 -> 27; int8 182 -> 308).
 //   A row tile's keys are shared by one wave up to 128 of them, else by four (80 x 58 keys, 12 heads: 6.0 against 8.0 us; 100 x 500: 20.4 against
-//   19.1), and by as many workgroups as give every CU two, none with less than 512 keys (1 x 131071 keys, 8 kv heads of 128, int8: 67 us in 64
+//   19.1), and by as many workgroups as give every CU two, none with less than 512 keys (1 x 131071 keys, 8 kv heads of 128, int8: 63 us in 64
 //   shares; 8 x 2000 keys: 15 us in 3 shares of 667, 17 in 7 of 286).
 //   Large tiles that leave a CU one workgroup get twice the waves, half the keys each (8 x 200 tokens over 712 keys, 12 heads: 28.4 -> 20.5 us; where
 //   CUs have two anyway it costs 5 %), and are shared out until every CU has that one (1 x 500 over 4000 33.6 -> 29.6; two a CU: twice the sums to
