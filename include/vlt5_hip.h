@@ -739,9 +739,10 @@ int vlt5_kv_page_read(const vlt5_paged_kv* c, const vlt5_paged_seqs* q, int T, v
  * key that lies `dist` positions back, the last entry for every larger dist -- T5's bucketed bias of a decoder as a function of the
  * distance.  A token that sees no key gets zeros and lse -inf.  What a token does not see may hold anything: keys behind the last one, and
  * keys that `causal` masks, whose values, finite or not, reach only the tokens that see them (an 8-bit value whose scale is not finite shows
- * in all of a token that sees it).  lse (optional) f32 [n_tok][H].  max_kv: about the longest kv_lens (0, or more than the table's width =
- * that width); it only decides how the work is split.  workspace: vlt5_paged_attn_workspace_bytes of the same desc (0: none needed, always
- * so where max_kv or the table's width is below VLT5_PAGED_SHARED_KV), 16-byte aligned, one per call in flight. */
+ * in all of a token that sees it, its lse included where the token is one of a chunk).  lse (optional) f32 [n_tok][H].  max_kv: about the
+ * longest kv_lens (0, or more than the table's width = that width); it only decides how the work is split.  workspace:
+ * vlt5_paged_attn_workspace_bytes of the same desc (0: none needed, always so where max_kv or the table's width is below
+ * VLT5_PAGED_SHARED_KV), 16-byte aligned, one per call in flight. */
 #define VLT5_PAGED_SHARED_KV 1024
 typedef struct {
     vlt5_paged_kv kv; vlt5_paged_seqs seqs;
